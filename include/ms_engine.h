@@ -413,6 +413,96 @@ int ms_prefill_tiles(const int32_t *seq_row0, const int32_t *seq_ntok, const int
                      const int32_t *seq_table_row, int32_t num_seqs, int32_t num_heads,
                      int32_t num_kv_heads, int32_t *tiles_out, int32_t capacity);
 
+/* ---- bounded caches: sliding windows, attention weights, eviction -------
+ * Four operators over the paged pools for sequences whose cache must not grow
+ * with their length (no counterpart in the reference, whose attention is
+ * causal over the whole cache).  Common to all of them:
+ *  - k_pool / v_pool [pool_blocks, num_kv_heads, 16, head_dim], 16-byte
+ *    aligned; block_tables [table_rows, max_blocks_per_seq]; num_heads /
+ *    num_kv_heads is 1, 2, 4, 7 or 8, head_dim 64 or 128, block_size 16;
+ *    q and out [rows, num_heads, head_dim], 16-byte aligned.
+ *  - They run on the current device, allocate nothing, and may be captured
+ *    into a graph; calls that may overlap need workspaces of their own.
+ *  - Host arguments out of range return cudaErrorInvalidValue before anything
+ *    is launched.  What lies in device memory is checked by the kernels: a row
+ *    (tile) whose context, positions or table row are out of range is skipped,
+ *    its outputs stay as they were; a page id outside [0, pool_blocks) is
+ *    never dereferenced, and the row that names it gets an unspecified result.
+ *    Both set bit 2 of the status word that ms_kernel_status returns.
+ *  - Table entries of pages that hold no key any row sees are not read, so the
+ *    pages behind a window may have been freed or reused.  Keys that no row of
+ *    a call's row (tile) sees may hold anything, NaN included; keys that some
+ *    row of a tile sees must be finite for all of its rows. */
+
+/* K3w: K3 with a sliding window and sink tokens.  Row t, at position p =
+ * row_ctx[t] - 1, attends to the keys j <= p with p - j < window or j < sinks
+ * (window = 0: to all j <= p); a row with row_ctx[t] = 0 gets zeros.
+ * row_table may be NULL (row t uses table row t; table_rows >= num_rows).
+ * Softmax in f32, one rounding of the result.  One launch, no workspace. */
+int ms_launch_window_attention(const void *q, const void *k_pool, const void *v_pool, int64_t pool_blocks,
+                               const int32_t *block_tables, int32_t table_rows, int32_t max_blocks_per_seq,
+                               const int32_t *row_table, const int32_t *row_ctx, int32_t num_rows,
+                               int32_t max_ctx, int32_t window, int32_t sinks, void *out, int32_t num_heads,
+                               int32_t num_kv_heads, int32_t head_dim, int32_t block_size, float scale,
+                               int32_t dtype, void *stream);
+
+/* K3pw: K3p with the same window and sinks, bf16 / f16; tiles as for
+ * ms_launch_paged_prefill (ms_prefill_tiles): the row at position p of a tile
+ * attends to the keys j <= p with p - j < window or j < sinks. */
+int ms_launch_window_prefill(const void *q, const void *k_pool, const void *v_pool, int64_t pool_blocks,
+                             const int32_t *block_tables, int32_t table_rows, int32_t max_blocks_per_seq,
+                             const int32_t *tiles, int32_t num_tiles, int32_t window, int32_t sinks, void *out,
+                             int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                             float scale, int32_t dtype, void *stream);
+
+/* K3a: K3 that also adds each key's softmax weight, summed over the query
+ * heads of its kv head, to weight_sum[table row][kv head][j] (f32 [table_rows,
+ * num_kv_heads, weight_stride], weight_stride >= max_ctx; slots from the
+ * row's context on are left as they are).  The caller zeroes a sequence's
+ * sums when it admits it.  A table row may appear once per call; a second row
+ * that names it is skipped and flagged.  Sums are taken in a fixed order:
+ * equal calls give equal bits.  workspace: ms_attention_weights_workspace_bytes. */
+int64_t ms_attention_weights_workspace_bytes(int32_t num_rows, int32_t num_heads, int32_t max_ctx);
+int ms_launch_attention_weights(const void *q, const void *k_pool, const void *v_pool, int64_t pool_blocks,
+                                const int32_t *block_tables, int32_t table_rows, int32_t max_blocks_per_seq,
+                                const int32_t *row_table, const int32_t *row_ctx, int32_t num_rows,
+                                int32_t max_ctx, void *out, float *weight_sum, int64_t weight_stride,
+                                int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                                float scale, void *workspace, int64_t workspace_bytes, int32_t dtype,
+                                void *stream);
+
+/* K7: eviction.  Each listed sequence keeps `keep` of its n = row_ctx[t] slots
+ * per kv head, in place, in slots [0, keep); the caller then goes on with a
+ * context of min(n, keep) (attention does not depend on the order of the
+ * slots) and may free the pages behind it.
+ *  - Slot j holds position pos_in[table row][kv head][j] for j < row_known[t]
+ *    (slots an earlier eviction placed) and row_next[t] - n + j from there on
+ *    (tokens appended since), row_next[t] = tokens the sequence has seen.
+ *    row_known may be NULL: 0, pos_in is then not read and may be NULL.
+ *  - Kept are the slots with position < sinks or >= row_next[t] - recent, and
+ *    of the others those with the largest weight_in[table row][kv head][j],
+ *    the lowest slot first among equals (-0 = 0; NaN ranks above infinity).
+ *    sinks + recent <= keep.
+ *  - A kept slot below keep stays.  The kept slots from keep on, in order,
+ *    move into the evicted slots below keep, in order: K and V rows, weight
+ *    and position.  With n <= keep nothing moves.
+ *  - weight_out[0, min(n, keep)) and pos_out get the kept slots' weights and
+ *    positions, weight_out[keep, n) zeros; the rest is left as it was.
+ *    weight_out may be weight_in and pos_out may be pos_in.
+ * weight_* f32 and pos_* int32 [table_rows, num_kv_heads, stride], stride >=
+ * max_ctx, max_ctx <= 49152.  A table row may appear once per call, and the
+ * listed sequences must own their pages: a page two of them share (a cached
+ * prefix) would be overwritten for both.  workspace:
+ * ms_evict_workspace_bytes. */
+int64_t ms_evict_workspace_bytes(int32_t num_rows, int32_t num_kv_heads, int32_t max_ctx);
+int ms_launch_evict(void *k_pool, void *v_pool, int64_t pool_blocks, const int32_t *block_tables,
+                    int32_t table_rows, int32_t max_blocks_per_seq, const int32_t *row_table,
+                    const int32_t *row_ctx, const int32_t *row_next, const int32_t *row_known,
+                    int32_t num_rows, int32_t max_ctx, int32_t keep, int32_t sinks, int32_t recent,
+                    const float *weight_in, float *weight_out, const int32_t *pos_in, int32_t *pos_out,
+                    int64_t stride, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                    void *workspace, int64_t workspace_bytes, int32_t dtype, void *stream);
+
 /* Status of the kernels launched without an engine on `device`: the
  * prototype-compatible launchers below, ms_launch_sample, and
  * ms_launch_paged_attention / ms_launch_paged_prefill (which use it when their

@@ -78,6 +78,41 @@ int prefill_tokens_per_tile(int group);
 // tokens; returns the tile count or -1 if capacity is exceeded.
 int build_prefill_tiles(const int32_t *seq_row0, const int32_t *seq_ntok, const int32_t *seq_start,
                         const int32_t *seq_trow, int num_seqs, int group, int32_t *tiles_out, int capacity);
+// K3w / K3pw / K3a (ms_window.cu): attention of rows or tiles over a bounded
+// part of the cache; see ms_launch_window_attention and its neighbours.
+struct WindowArgs {
+  const void *q;
+  const void *k_pool;
+  const void *v_pool;
+  int64_t pool_blocks;
+  const int32_t *block_tables;
+  int table_rows;
+  int max_blocks_per_seq;
+  const int32_t *row_table;  // rows
+  const int32_t *row_ctx;
+  int num_rows;
+  int max_ctx;
+  const int32_t *tiles;      // or tiles
+  int num_tiles;
+  int window;                // 0: every key
+  int sinks;
+  void *out;
+  float *weight_sum;         // rows: accumulate the softmax weights
+  int64_t weight_stride;
+  void *workspace;
+  int64_t workspace_bytes;
+  int num_heads;
+  int num_kv_heads;
+  int head_dim;
+  int block_size;
+  float scale;
+  int dtype;
+  unsigned *status;          // null: the standalone status word
+};
+cudaError_t launch_window_attention(const WindowArgs &a, cudaStream_t stream);
+cudaError_t launch_window_prefill(const WindowArgs &a, cudaStream_t stream);
+int64_t attention_weights_workspace_bytes(int num_rows, int num_heads, int max_ctx);
+
 int choose_partition_blocks(int num_rows, int num_kv_heads, int max_ctx, long long total_blocks);
 int64_t attention_workspace_bytes(int num_rows, int num_heads, int max_ctx, int part_blocks);
 
