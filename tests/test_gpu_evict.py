@@ -147,7 +147,6 @@ def test_ties_and_special_weights(kind):
 
 
 @pytest.mark.parametrize("ctx,keep", [([5000, 4097], 4096), ([20000], 513), ([9000, 33], 8999)])
-                                      ([140001], 1000)])
 def test_long(ctx, keep):
     s = state(ctx, 2, 64, torch.float16, keep)
     run(s, keep, 4, min(200, keep // 2), ctx, None, torch.float16, True)
