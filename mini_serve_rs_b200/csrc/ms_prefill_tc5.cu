@@ -40,6 +40,12 @@
 // (8 slots of 16 KB for D = 64), one CTA per SM; TMEM: 512 columns (per half
 // S/P 128 + O D).
 //
+// The windowed build (WIN, K3pw) visits only the pages that some row of the
+// tile sees, packed into one run of virtual keys (sink pages, then the
+// window's), so a few sinks do not cost a group of their own and the window
+// starts at a page, not at a group.  Groups that reach below the last row's
+// window or past the first row's position take the two-sided mask.
+//
 // Every wait is bounded (mbarrier polls that also watch a CTA abort flag);
 // on expiry the CTA records kStatusWaitTimeout, drains its MMAs and copies
 // (bounded), frees TMEM and returns.
@@ -49,7 +55,7 @@
 #include <mutex>
 #include <type_traits>
 
-#include "ms_attention_common.cuh"
+#include "ms_window.cuh"
 
 namespace ms {
 namespace attn {
@@ -161,6 +167,10 @@ struct Prefill5Params {
   int max_blocks_per_seq;
   int num_kv_heads;
   float qscale;
+  // windowed build only
+  int window, sinks;  // row at p sees j <= p with p - j < window or j < sinks
+  int table_rows;
+  int64_t pool_blocks;
 };
 
 constexpr int kHalves = 2;  // query halves of 128 rows per CTA, sharing every K/V tile
@@ -216,6 +226,10 @@ __device__ __forceinline__ void exp2_poly2(float &y0, float &y1, float x0, float
   y0 = __int_as_float(__float_as_int(p0) + (__float_as_int(t0) << 23));
   y1 = __int_as_float(__float_as_int(p1) + (__float_as_int(t1) << 23));
 }
+// bits 0 .. n - 1 set (none for n <= 0, all from n = 32 on)
+__device__ __forceinline__ uint32_t keys_below(int n) {
+  return n <= 0 ? 0u : 0xffffffffu >> (32 - min(n, 32));
+}
 __device__ __forceinline__ float ex2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -254,7 +268,7 @@ __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.
 
 constexpr int kThreads5 = 320;  // 2 x 4 softmax warps (one group of 4 per query half), the MMA warp, the copy warp
 
-template <typename T, int D, int G>
+template <typename T, int D, int G, bool WIN>
 __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill5Params p) {
   constexpr int RPT = RowsPerTok5<G>::value;
   constexpr int TPH = kRows / RPT;     // tokens per query half
@@ -279,8 +293,27 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
   const int row0 = p.tiles[tile * 4 + 0], nrows = p.tiles[tile * 4 + 1];
   const int pos0 = p.tiles[tile * 4 + 2], trow = p.tiles[tile * 4 + 3];
   const int32_t *table = p.block_tables + size_t(trow) * p.max_blocks_per_seq;
-  const int kv_len = pos0 + nrows;
-  const int npages = (kv_len + kBS - 1) / kBS;
+  int kv_len = pos0 + nrows;
+  int npages = (kv_len + kBS - 1) / kBS;
+  // Windowed build: the pages that some row of the tile sees, sink pages first, are one run of
+  // virtual keys; from here on a key is its virtual index (positions move by `shift`).  Keys in
+  // [dead0, dead1) and from kv_len on lie in those pages but no row sees them.
+  [[maybe_unused]] VisiblePages vis;
+  int shift = 0, dead0 = 0, dead1 = 0;
+  if constexpr (WIN) {
+    if (row0 < 0 || nrows < 0 || nrows > kHalves * TPH || pos0 < 0 || trow < 0 || trow >= p.table_rows ||
+        pos0 > p.max_blocks_per_seq * kBS - nrows) {
+      if (t == 0) atomicOr(p.status, kStatusBadIndex);
+      return;
+    }
+    if (nrows == 0) return;
+    vis = VisiblePages(pos0, kv_len, p.window, p.sinks);
+    shift = vis.shift();
+    npages = vis.count;
+    kv_len += shift;
+    dead1 = VisiblePages::lowest_key(pos0, p.window) + shift;
+    dead0 = min(p.sinks, dead1);
+  }
   const int ngroups = (kv_len + kKeys - 1) / kKeys;
   const int ntiles = 2 * ngroups;  // ring order K0 V0 K1 V1 ...: K(g) is tile 2g, V(g) tile 2g + 1
   // groups each query half attends to (its last token's causal range); half 1 may be empty
@@ -288,7 +321,7 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
 #pragma unroll
   for (int h = 0; h < kHalves; ++h) {
     const int last = min(nrows, (h + 1) * TPH);  // tokens up to the end of half h
-    ng[h] = last > h * TPH ? (pos0 + last + kKeys - 1) / kKeys : 0;
+    ng[h] = last > h * TPH ? (pos0 + last + shift + kKeys - 1) / kKeys : 0;
   }
 
   if (t == 0) {
@@ -354,8 +387,16 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
     // ---- softmax: row rt of query half qh ----
     const uint32_t lane_off = uint32_t((warp & 3) * 32) << 16;
     const uint32_t tm_s = tmem + qh * 256, tm_o = tm_s + kKeys;
-    const int pos_first = pos0 + qh * TPH;            // first position of this half
-    const int pos = rvalid ? pos0 + tok : pos_first;  // padding rows copy the half's first row mask
+    const int pos_first = pos0 + shift + qh * TPH;            // first position of this half
+    const int pos = rvalid ? pos0 + shift + tok : pos_first;  // padding rows copy the half's first row mask
+    // windowed build: the first key of this row's window, and of the half's last row (keys below
+    // it take the mask, unless the sinks reach that far)
+    int lo = 0, lo_last = 0;
+    if constexpr (WIN) {
+      lo = VisiblePages::lowest_key(pos - shift, p.window) + shift;
+      lo_last = VisiblePages::lowest_key(pos0 + min(nrows, (qh + 1) * TPH) - 1, p.window) + shift;
+      if (lo_last <= p.sinks) lo_last = 0;
+    }
     const float c = p.qscale;
     // the lowest half that attends to the last group zeroes its V rows past the sequence
     const bool zeroes_v = ng_q == ngroups && (qh == 0 || ng[0] < ngroups);
@@ -370,12 +411,24 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
       // pass 1 takes the row max, pass 2 turns the scores into P.  Only groups that reach past
       // the half's first position take the causal mask (a CTA-uniform branch).
       const int key0 = g * kKeys;
-      const bool diag = key0 + kKeys - 1 > pos_first;
+      const bool diag = key0 + kKeys - 1 > pos_first || (WIN && key0 < lo_last);
       constexpr int NC = kKeys / 32;
-      auto score = [&](auto masked, const uint32_t *cur, int k, int i) {
+      // bits: windowed build, the visible keys of the 32-column chunk (one register instead of
+      // two bounds and two compares a score, which spilled)
+      auto score = [&](auto masked, const uint32_t *cur, int k, int i, uint32_t bits) {
         const float v = __uint_as_float(cur[i]);
-        if constexpr (decltype(masked)::value) return key0 + 32 * k + i <= pos ? v : -INFINITY;
+        if constexpr (decltype(masked)::value) {
+          if constexpr (WIN) return bits & (1u << i) ? v : -INFINITY;
+          return key0 + 32 * k + i <= pos ? v : -INFINITY;
+        }
         return v;
+      };
+      auto visible_bits = [&](auto masked, int k) -> uint32_t {
+        if constexpr (WIN && decltype(masked)::value) {
+          const int base = key0 + 32 * k;
+          return keys_below(pos + 1 - base) & (~keys_below(lo - base) | keys_below(p.sinks - base));
+        }
+        return 0u;
       };
       auto row_max = [&](auto masked) {
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -386,9 +439,10 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
           tmem_wait_ld();
           const uint32_t *cur = (k & 1) ? cb : ca;
           if (k + 1 < NC) tmem_ld32_async(tm_s + lane_off + 32 * (k + 1), (k & 1) ? ca : cb);
+          const uint32_t bits = visible_bits(masked, k);
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            mx[i & 3] = max3f(mx[i & 3], score(masked, cur, k, 2 * i), score(masked, cur, k, 2 * i + 1));
+            mx[i & 3] = max3f(mx[i & 3], score(masked, cur, k, 2 * i, bits), score(masked, cur, k, 2 * i + 1, bits));
         }
         return fmaxf(max3f(mx[0], mx[1], mx[2]), mx[3]);
       };
@@ -416,7 +470,8 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
           tmem_st32(tm_o + lane_off + c0, o);
         }
       }
-      const float negm = -m_run;
+      // a windowed row may have seen nothing yet: -inf scores then give 2^-inf = 0
+      const float negm = WIN && m_run == -INFINITY ? 0.f : -m_run;
       float ps[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       // P of chunk k (16 columns of value pairs) goes to columns [16k, 16k + 16): over S chunks
       // already read, never over the chunk loading next.  Two scores per packed FMA and add.
@@ -428,12 +483,15 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
           tmem_wait_ld();
           const uint32_t *cur = (k & 1) ? cb : ca;
           if (k + 1 < NC) tmem_ld32_async(tm_s + lane_off + 32 * (k + 1), (k & 1) ? ca : cb);
+          const uint32_t bits = visible_bits(masked, k);
           uint32_t pk[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             float x0, x1, a, b;
-            ffma2(x0, x1, score(masked, cur, k, 2 * i), score(masked, cur, k, 2 * i + 1), c, negm);
-            if ((i & 7) < kExp2OnFma) {  // a share of the exponentials off the transcendental unit
+            ffma2(x0, x1, score(masked, cur, k, 2 * i, bits), score(masked, cur, k, 2 * i + 1, bits), c, negm);
+            // (the polynomial gives 1e-38 for a masked score: the windowed build, whose masked V
+            // rows may be another row's live ones, keeps masked groups on ex2 and its exact 0)
+            if ((i & 7) < kExp2OnFma && !(WIN && decltype(masked)::value)) {  // a share of the exponentials off the transcendental unit
               exp2_poly2(a, b, x0, x1);
             } else {
               a = ex2_approx(x0);
@@ -452,17 +510,27 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
       l_run = l_run * alpha + psum;
       // the last group's V rows past the sequence (stale, or pages never loaded) -> 0
       const int vk = kv_len - key0;
-      if (zeroes_v && g == ngroups - 1 && vk < kKeys) {
+      int z0 = kKeys, z1 = kKeys;  // keys [z0, z1) of the group
+      if (zeroes_v && g == ngroups - 1 && vk < kKeys) z0 = vk;
+      // windowed build: and the dead keys before the window (half 0 attends to every group they
+      // reach, and its PV is issued first); where both meet in one group, in two rounds
+      const int y0 = max(0, dead0 - key0), y1 = min(kKeys, dead1 - key0);
+      const bool dead = WIN && qh == 0 && y0 < y1;
+      if (z0 < z1 || dead) {
         const int iv = 2 * g + 1;
         if (!__all_sync(kFull, wait_or_abort(&full[iv % NSLOT], (iv / NSLOT) & 1, &abort_s))) {
           abort_s = 1;
           break;
         }
         unsigned char *vst = ring + (iv % NSLOT) * TILE;
-        for (int i = rt; i < (kKeys - vk) * 8 * NDH; i += kRows) {
-          const int dh = i / ((kKeys - vk) * 8), rem = i % ((kKeys - vk) * 8);
-          *reinterpret_cast<uint4 *>(vst + dh * HALF + (vk + rem / 8) * 128 + (rem % 8) * 16) = make_uint4(0, 0, 0, 0);
-        }
+        auto zero_rows = [&](int r0, int r1) {
+          for (int i = rt; i < (r1 - r0) * 8 * NDH; i += kRows) {
+            const int dh = i / ((r1 - r0) * 8), rem = i % ((r1 - r0) * 8);
+            *reinterpret_cast<uint4 *>(vst + dh * HALF + (r0 + rem / 8) * 128 + (rem % 8) * 16) = make_uint4(0, 0, 0, 0);
+          }
+        };
+        if (z0 < z1) zero_rows(z0, z1);
+        if (dead) zero_rows(y0, y1);
         fence_proxy_async();
       }
       tc_fence_before();
@@ -555,7 +623,16 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
     // visible to the tensor core (fence.proxy.async) after its wait.
     constexpr int CPR = D / 8, RPI = 32 / CPR, IPP = kBS / RPI;  // chunks per row, rows per instruction, per page
     const int cc = lane % CPR, dh = cc >> 3, ch = cc & 7, r0 = lane / CPR;
-    auto table_at = [&](int i) { return i < npages ? table[i] : 0; };
+    auto table_at = [&](int i) {
+      if (i >= npages) return 0;
+      if constexpr (WIN) {
+        const int page = table[vis.page_at(i)];
+        if (page >= 0 && page < p.pool_blocks) return page;
+        atomicOr(p.status, kStatusBadIndex);
+        return 0;
+      }
+      return table[i];
+    };
     int kw = 0, vw = 0;
     int kcur = table_at(lane), vcur = kcur, knxt = table_at(32 + lane), vnxt = knxt;
     int issued = 0;
@@ -657,9 +734,9 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
   if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS));
 }
 
-template <typename T, int D, int G>
+template <typename T, int D, int G, bool WIN>
 cudaError_t launch_t5(const Prefill5Params &p, int num_tiles, cudaStream_t stream) {
-  auto kern = paged_prefill_tc5_kernel<T, D, G>;
+  auto kern = paged_prefill_tc5_kernel<T, D, G, WIN>;
   const size_t smem = Ring5<D>::kSmem;
   static std::atomic<bool> attr_done[64];  // zero-initialised (static storage)
   int dev = 0;
@@ -675,16 +752,28 @@ cudaError_t launch_t5(const Prefill5Params &p, int num_tiles, cudaStream_t strea
   return cudaGetLastError();
 }
 
-template <typename T, int D>
+template <typename T, int D, bool WIN>
 cudaError_t t5_group(const Prefill5Params &p, int group, int num_tiles, cudaStream_t stream) {
   switch (group) {
-    case 1: return launch_t5<T, D, 1>(p, num_tiles, stream);
-    case 2: return launch_t5<T, D, 2>(p, num_tiles, stream);
-    case 4: return launch_t5<T, D, 4>(p, num_tiles, stream);
-    case 7: return launch_t5<T, D, 7>(p, num_tiles, stream);
-    case 8: return launch_t5<T, D, 8>(p, num_tiles, stream);
+    case 1: return launch_t5<T, D, 1, WIN>(p, num_tiles, stream);
+    case 2: return launch_t5<T, D, 2, WIN>(p, num_tiles, stream);
+    case 4: return launch_t5<T, D, 4, WIN>(p, num_tiles, stream);
+    case 7: return launch_t5<T, D, 7, WIN>(p, num_tiles, stream);
+    case 8: return launch_t5<T, D, 8, WIN>(p, num_tiles, stream);
     default: return cudaErrorInvalidValue;
   }
+}
+
+template <bool WIN>
+cudaError_t t5_type(const Prefill5Params &p, int dtype, int head_dim, int group, int num_tiles, cudaStream_t stream) {
+  if (dtype == MS_DTYPE_BF16) {
+    if (head_dim == 128) return t5_group<__nv_bfloat16, 128, WIN>(p, group, num_tiles, stream);
+    if (head_dim == 64) return t5_group<__nv_bfloat16, 64, WIN>(p, group, num_tiles, stream);
+  } else if (dtype == MS_DTYPE_F16) {
+    if (head_dim == 128) return t5_group<__half, 128, WIN>(p, group, num_tiles, stream);
+    if (head_dim == 64) return t5_group<__half, 64, WIN>(p, group, num_tiles, stream);
+  }
+  return cudaErrorInvalidValue;
 }
 
 }  // namespace
@@ -699,7 +788,7 @@ cudaError_t launch_prefill_tc5(const void *q, void *out, const int32_t *block_ta
                                float scale, unsigned *status, int dtype, const void *k_pool, const void *v_pool,
                                cudaStream_t stream) {
   if ((reinterpret_cast<uintptr_t>(k_pool) | reinterpret_cast<uintptr_t>(v_pool)) & 15) return cudaErrorInvalidValue;
-  Prefill5Params p;
+  Prefill5Params p{};
   p.q = q;
   p.k_pool = k_pool;
   p.v_pool = v_pool;
@@ -710,14 +799,26 @@ cudaError_t launch_prefill_tc5(const void *q, void *out, const int32_t *block_ta
   p.max_blocks_per_seq = max_blocks_per_seq;
   p.num_kv_heads = num_kv_heads;
   p.qscale = scale * kLog2e;
-  if (dtype == MS_DTYPE_BF16) {
-    if (head_dim == 128) return t5_group<__nv_bfloat16, 128>(p, group, num_tiles, stream);
-    if (head_dim == 64) return t5_group<__nv_bfloat16, 64>(p, group, num_tiles, stream);
-  } else if (dtype == MS_DTYPE_F16) {
-    if (head_dim == 128) return t5_group<__half, 128>(p, group, num_tiles, stream);
-    if (head_dim == 64) return t5_group<__half, 64>(p, group, num_tiles, stream);
-  }
-  return cudaErrorInvalidValue;
+  return t5_type<false>(p, dtype, head_dim, group, num_tiles, stream);
+}
+
+cudaError_t launch_window_prefill_tc5(const WindowArgs &a, cudaStream_t stream) {
+  Prefill5Params p{};
+  p.q = a.q;
+  p.k_pool = a.k_pool;
+  p.v_pool = a.v_pool;
+  p.out = a.out;
+  p.block_tables = a.block_tables;
+  p.tiles = a.tiles;
+  p.status = a.status;
+  p.max_blocks_per_seq = a.max_blocks_per_seq;
+  p.num_kv_heads = a.num_kv_heads;
+  p.qscale = a.scale * kLog2e;
+  p.window = a.window;
+  p.sinks = a.sinks;
+  p.table_rows = a.table_rows;
+  p.pool_blocks = a.pool_blocks;
+  return t5_type<true>(p, a.dtype, a.head_dim, a.num_heads / a.num_kv_heads, a.num_tiles, stream);
 }
 
 }  // namespace attn

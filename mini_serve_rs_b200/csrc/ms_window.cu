@@ -6,7 +6,9 @@
 // the whole cache with W[j] += sum over the kv head's query heads of key j's
 // softmax weight (K3a).
 //
-// One CTA per (row, kv head); its warps take the visible keys in turn, a lane
+// K3pw is the windowed build of the tcgen05 prefill kernel
+// (ms_prefill_tc5.cu); this file checks its arguments.  Single tokens:
+// one CTA per (row, kv head); its warps take the visible keys in turn, a lane
 // holding head_dim / 32 dims, every query head of the kv head served by one
 // read of K and V.  Softmax is online in base 2; the warps merge in shared
 // memory.  K3a keeps the raw scores in the workspace and turns them into
@@ -22,7 +24,6 @@ struct RowsParams {
   WindowArgs a;
   int group;
   float qscale;
-  int tile_tokens;
   unsigned *status;
 };
 
@@ -32,22 +33,8 @@ __global__ void __launch_bounds__(128) window_rows_kernel(RowsParams p) {
   const WindowArgs &a = p.a;
   const int kvh = blockIdx.y, G = p.group;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int row, ctx, trow;
-  bool ok = true;
-  if (a.tiles) {
-    const int tile = blockIdx.x / p.tile_tokens, i = blockIdx.x % p.tile_tokens;
-    const int row0 = a.tiles[4 * tile], nrows = a.tiles[4 * tile + 1], pos0 = a.tiles[4 * tile + 2];
-    trow = a.tiles[4 * tile + 3];
-    ok = row0 >= 0 && nrows >= 0 && nrows <= p.tile_tokens && pos0 >= 0 && pos0 <= a.max_ctx - nrows;
-    if (ok && i >= nrows) return;
-    row = row0 + i;
-    ctx = pos0 + i + 1;
-  } else {
-    row = blockIdx.x;
-    ctx = a.row_ctx[row];
-    trow = a.row_table ? a.row_table[row] : row;
-    ok = ctx >= 0 && ctx <= a.max_ctx;
-  }
+  const int row = blockIdx.x, ctx = a.row_ctx[row], trow = a.row_table ? a.row_table[row] : row;
+  bool ok = ctx >= 0 && ctx <= a.max_ctx;
   ok = ok && trow >= 0 && trow < a.table_rows;
   if (a.weight_sum && table_row_repeated(a.row_table, row, trow)) ok = false;
   if (!ok) {
@@ -141,35 +128,33 @@ __global__ void __launch_bounds__(128) window_rows_kernel(RowsParams p) {
 }
 
 template <typename T>
-cudaError_t launch_rows(const RowsParams &p, long long rows, cudaStream_t stream) {
-  if (rows > 0x7fffffffLL) return cudaErrorInvalidValue;
-  const dim3 grid(unsigned(rows), p.a.num_kv_heads);
+cudaError_t launch_rows(const RowsParams &p, cudaStream_t stream) {
+  const dim3 grid(p.a.num_rows, p.a.num_kv_heads);
   if (p.a.head_dim == 128) window_rows_kernel<T, 128><<<grid, 128, 0, stream>>>(p);
   else window_rows_kernel<T, 64><<<grid, 128, 0, stream>>>(p);
   return cudaGetLastError();
 }
 
-cudaError_t launch_checked(const WindowArgs &a, long long rows, int tile_tokens, cudaStream_t stream) {
+cudaError_t launch_checked(const WindowArgs &a, cudaStream_t stream) {
   RowsParams p{};
   p.a = a;
   p.group = a.num_heads / a.num_kv_heads;
   p.qscale = a.scale * attn::kLog2e;
-  p.tile_tokens = tile_tokens;
   p.status = a.status;
   if (!p.status) {
     const cudaError_t e = standalone_status_word(&p.status);
     if (e != cudaSuccess) return e;
   }
-  if (a.dtype == MS_DTYPE_F32) return launch_rows<float>(p, rows, stream);
-  if (a.dtype == MS_DTYPE_BF16) return launch_rows<__nv_bfloat16>(p, rows, stream);
-  return launch_rows<__half>(p, rows, stream);
+  if (a.dtype == MS_DTYPE_F32) return launch_rows<float>(p, stream);
+  if (a.dtype == MS_DTYPE_BF16) return launch_rows<__nv_bfloat16>(p, stream);
+  return launch_rows<__half>(p, stream);
 }
 
 bool common_ok(const WindowArgs &a) {
   return head_layout_ok(a.num_heads, a.num_kv_heads, a.head_dim, a.block_size, a.dtype) && a.num_kv_heads <= 65535 &&
          pools_ok(a.k_pool, a.v_pool, a.pool_blocks, a.num_kv_heads, a.block_tables, a.table_rows,
                   a.max_blocks_per_seq) &&
-         ptr16(a.q) && ptr16(a.out) && a.window >= 0 && a.sinks >= 0;
+         ptr16(a.q) && ptr16(a.out) && a.scale > 0.f && a.scale < INFINITY && a.window >= 0 && a.sinks >= 0;
 }
 
 }  // namespace
@@ -183,7 +168,7 @@ cudaError_t launch_window_attention(const WindowArgs &a, cudaStream_t stream) {
   if (a.weight_sum && (a.weight_stride < a.max_ctx || !ptr16(a.workspace) ||
                        a.workspace_bytes < attention_weights_workspace_bytes(a.num_rows, a.num_heads, a.max_ctx)))
     return cudaErrorInvalidValue;
-  return launch_checked(a, a.num_rows, 1, stream);
+  return launch_checked(a, stream);
 }
 
 cudaError_t launch_window_prefill(const WindowArgs &args, cudaStream_t stream) {
@@ -191,9 +176,12 @@ cudaError_t launch_window_prefill(const WindowArgs &args, cudaStream_t stream) {
   if (a.num_tiles < 0) return cudaErrorInvalidValue;
   if (a.num_tiles == 0) return cudaSuccess;
   if (!common_ok(a) || !a.tiles || a.dtype == MS_DTYPE_F32 || a.num_tiles > 65535) return cudaErrorInvalidValue;
-  a.max_ctx = a.max_blocks_per_seq * attn::kBS;
-  const int tpt = prefill_tokens_per_tile(a.num_heads / a.num_kv_heads);
-  return launch_checked(a, (long long)a.num_tiles * tpt, tpt, stream);
+  if (!attention_tc_available(a.dtype, a.head_dim, a.num_heads / a.num_kv_heads)) return cudaErrorInvalidValue;
+  if (!a.status) {
+    const cudaError_t e = standalone_status_word(&a.status);
+    if (e != cudaSuccess) return e;
+  }
+  return attn::launch_window_prefill_tc5(a, stream);
 }
 
 int64_t attention_weights_workspace_bytes(int num_rows, int num_heads, int max_ctx) {

@@ -16,6 +16,7 @@ struct VisiblePages {
   int sink_pages = 0;
   int first_page = 0;
   int count = 0;
+  VisiblePages() = default;
   __device__ __forceinline__ VisiblePages(int first_pos, int end, int window, int sinks) {
     const int low = lowest_key(first_pos, window);
     first_page = low / attn::kBS;
@@ -56,5 +57,10 @@ inline bool pools_ok(const void *k_pool, const void *v_pool, int64_t pool_blocks
          max_blocks_per_seq > 0 && max_blocks_per_seq <= (1 << 26) && num_kv_heads > 0 &&
          pool_blocks <= ((int64_t(1) << 31) - 1) / num_kv_heads;
 }
+
+namespace attn {
+// windowed build of the tcgen05 prefill kernel (ms_prefill_tc5.cu); arguments checked, status set
+cudaError_t launch_window_prefill_tc5(const WindowArgs &a, cudaStream_t stream);
+}  // namespace attn
 
 }  // namespace ms

@@ -47,7 +47,8 @@ def evict(**kw):
 COMMON = [dict(k=None), dict(v=None), dict(tables=None), dict(k=P + 8), dict(v=P + 8), dict(pool=0), dict(pool=-1),
           dict(pool=1 << 31), dict(pool=1 << 40), dict(table_rows=0), dict(blocks=0), dict(blocks=-4), dict(d=96), dict(d=0),
           dict(bs=32), dict(dtype=3), dict(dtype=-1), dict(hkv=0), dict(n=-1), dict(sinks=-1)]
-HEADS = [dict(hq=0), dict(hq=24), dict(hq=17), dict(hq=128), dict(q=None), dict(q=P + 8), dict(out=None), dict(out=P + 4)]
+HEADS = [dict(hq=0), dict(hq=24), dict(hq=17), dict(hq=128), dict(q=None), dict(q=P + 8), dict(out=None), dict(out=P + 4), dict(scale=0.0),
+         dict(scale=-0.1), dict(scale=float("nan")), dict(scale=float("inf"))]
 
 
 @pytest.mark.parametrize("bad", COMMON + HEADS + [
