@@ -26,37 +26,6 @@
 namespace ms {
 namespace attn {
 
-// ---- transposed butterfly: NVP partial values per lane -> NVP/32 totals ------
-// After the call, lane L holds in v[j] the warp-wide sum of original index
-// L * (NVP/32) + j.
-template <int N, int OFF> struct Butterfly {
-  static __device__ __forceinline__ void run(float *v, int lane) {
-    const bool up = (lane & OFF) != 0;
-#pragma unroll
-    for (int j = 0; j < N / 2; ++j) {
-      float send = up ? v[j] : v[j + N / 2];
-      float keep = up ? v[j + N / 2] : v[j];
-      v[j] = keep + __shfl_xor_sync(kFull, send, OFF);
-    }
-    Butterfly<N / 2, OFF / 2>::run(v, lane);
-  }
-};
-template <int N> struct Butterfly<N, 0> {
-  static __device__ __forceinline__ void run(float *, int) {}
-};
-
-template <typename T, int D> struct TileLoad {
-  static constexpr int DPL = D / 32;
-  static __device__ __forceinline__ void load(const T *row, int lane, float (&o)[DPL]) {
-    if constexpr (DPL == 4) {
-      Vec4<T>::load(row + lane * 4, o);
-    } else {
-      Vec2<T>::load(row + lane * 2, o);
-    }
-  }
-};
-
-
 template <typename T, int D, int G, int NSTAGE>
 __global__ void __launch_bounds__(kWarps * 32) paged_attention_kernel(Params p) {
   constexpr int DPL = D / 32;
@@ -357,6 +326,11 @@ __device__ unsigned g_status_scratch;
 // Test hook: >= 0 replaces the poll limit of the page-loop waits (ms_test_set_attention_wait_limit).
 std::atomic<int> g_test_wait_limit{-1};
 
+int page_wait_limit() {
+  const int test_limit = g_test_wait_limit.load(std::memory_order_relaxed);
+  return test_limit >= 0 ? test_limit : kWaitLimit;
+}
+
 }  // namespace attn
 
 cudaError_t standalone_status_word(unsigned **out) {
@@ -413,8 +387,7 @@ cudaError_t launch_paged_attention(const AttnArgs &a, cudaStream_t stream) {
   p.max_parts = (max_blk + a.part_blocks - 1) / a.part_blocks;
   if (p.max_parts > 65535) return cudaErrorInvalidValue;
   p.qscale = a.scale * attn::kLog2e;
-  const int test_limit = attn::g_test_wait_limit.load(std::memory_order_relaxed);
-  p.wait_limit = test_limit >= 0 ? test_limit : attn::kWaitLimit;
+  p.wait_limit = attn::page_wait_limit();
   p.status = a.status;
   if (p.status == nullptr) {
     cudaError_t e = standalone_status_word(&p.status);

@@ -121,6 +121,56 @@ __device__ __forceinline__ void mma_16816<__half>(float (&d)[4], const uint32_t 
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// ---- 16-bit tiles: 16 tokens x D as D / 64 swizzled boxes -----------------------
+constexpr int kHalfBytes = 16 * 64 * 2;  // one 16-token x 64-dim box of 16-bit elements
+
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<uint32_t *>(&v);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<uint32_t *>(&v);
+}
+
+// byte offset of (token, dim) inside one tile stored as D/64 boxes of
+// [16 tokens][64 dims] with the 128-byte swizzle (16-byte chunk ^ token % 8)
+__device__ __forceinline__ uint32_t tile_off(int token, int dim) {
+  const int dh = dim >> 6, c = (dim & 63) >> 3;
+  return uint32_t(dh * kHalfBytes + token * 128 + ((c ^ (token & 7)) << 4));
+}
+
+// ---- transposed butterfly: NVP partial values per lane -> NVP/32 totals ------
+// After the call, lane L holds in v[j] the warp-wide sum of original index
+// L * (NVP/32) + j.
+template <int N, int OFF> struct Butterfly {
+  static __device__ __forceinline__ void run(float *v, int lane) {
+    const bool up = (lane & OFF) != 0;
+#pragma unroll
+    for (int j = 0; j < N / 2; ++j) {
+      float send = up ? v[j] : v[j + N / 2];
+      float keep = up ? v[j + N / 2] : v[j];
+      v[j] = keep + __shfl_xor_sync(kFull, send, OFF);
+    }
+    Butterfly<N / 2, OFF / 2>::run(v, lane);
+  }
+};
+template <int N> struct Butterfly<N, 0> {
+  static __device__ __forceinline__ void run(float *, int) {}
+};
+
+template <typename T, int D> struct TileLoad {
+  static constexpr int DPL = D / 32;
+  static __device__ __forceinline__ void load(const T *row, int lane, float (&o)[DPL]) {
+    if constexpr (DPL == 4) {
+      Vec4<T>::load(row + lane * 4, o);
+    } else {
+      Vec2<T>::load(row + lane * 2, o);
+    }
+  }
+};
+
 // ---- epilogue: merge the CTA's warps, write the output or the partition ---------
 // mo [kWarps][G][D] (unnormalised O, relative to the warp's running max),
 // mm / ml [kWarps][G] (running max in base 2, running sum) are in shared
@@ -188,6 +238,9 @@ cudaError_t launch_combine(const Params &p, int num_rows, cudaStream_t stream) {
   combine_kernel<T, D, G><<<g2, (G * D < 1024 ? G * D : 1024), 0, stream>>>(p);
   return cudaGetLastError();
 }
+
+// Poll limit of the page-loop waits (kWaitLimit, or what ms_test_set_attention_wait_limit set).
+int page_wait_limit();
 
 // Tensor-core (mma.sync) build for 16-bit K/V; maps may be null (encoded per call).
 cudaError_t launch_attention_tc(const Params &p, const AttnArgs &a, int group, cudaStream_t stream);

@@ -33,25 +33,6 @@ namespace ms {
 namespace attn {
 namespace {
 
-constexpr int kHalfBytes = 16 * 64 * 2;  // one 16-token x 64-dim box of 16-bit elements
-
-template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
-template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
-  __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<uint32_t *>(&v);
-}
-template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
-  __half2 v = __floats2half2_rn(a, b);
-  return *reinterpret_cast<uint32_t *>(&v);
-}
-
-// byte offset of (token, dim) inside one tile stored as D/64 boxes of
-// [16 tokens][64 dims] with the 128-byte swizzle (16-byte chunk ^ token % 8)
-__device__ __forceinline__ uint32_t tile_off(int token, int dim) {
-  const int dh = dim >> 6, c = (dim & 63) >> 3;
-  return uint32_t(dh * kHalfBytes + token * 128 + ((c ^ (token & 7)) << 4));
-}
-
 template <typename T, int D, int G, int NSTAGE>
 __global__ void __launch_bounds__(kWarps * 32)
     paged_attention_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,

@@ -4,150 +4,604 @@
 //
 // for single tokens (K3w) and for the tiles of prompt chunks (K3pw), and over
 // the whole cache with W[j] += sum over the kv head's query heads of key j's
-// softmax weight (K3a).
+// softmax weight (K3a).  K3pw is the windowed build of the tcgen05 prefill
+// kernel (ms_prefill_tc5.cu); this file checks its arguments.
 //
-// K3pw is the windowed build of the tcgen05 prefill kernel
-// (ms_prefill_tc5.cu); this file checks its arguments.  Single tokens:
-// one CTA per (row, kv head); its warps take the visible keys in turn, a lane
-// holding head_dim / 32 dims, every query head of the kv head served by one
-// read of K and V.  Softmax is online in base 2; the warps merge in shared
-// memory.  K3a keeps the raw scores in the workspace and turns them into
-// weights once the row's maximum and sum are known.
+// Single tokens: bound by reading the visible K and V once, so the kernel is
+// built around keeping copies in flight.  A cluster of C CTAs serves one (row,
+// kv head); CTA c takes the c-th share of the row's visible pages (sink pages,
+// then the window's; the others are never touched), its 4 warps take the
+// share's pages in turn, each through a private ring of shared-memory stages
+// filled by TMA (no multicast) on per-stage mbarriers.  One read of K and V
+// serves all query heads of the kv head:
+//  * 16-bit: the heads are rows 0..G-1 of an m16 tile, S = Q K^T and O += P V
+//    as mma.sync.m16n8k16 on the swizzled tile (16 x 16 x D per page is far
+//    below one tcgen05 tile), online softmax in base 2 on the four scores a
+//    lane holds;
+//  * f32: a lane owns D / 32 dims; partial dot products of 16 tokens are
+//    reduced across the warp by a transposed butterfly.
+// The warps merge in shared memory, the CTAs of the cluster read one another's
+// maxima, sums and outputs there (distributed shared memory): one launch, no
+// workspace, and the split depends on the call's shape only, so equal calls
+// give equal bits.
+// K3a needs the row's final maximum and sum before a score becomes a weight:
+// each CTA writes its raw scores to the workspace (they stay in L2) and reads
+// them back once the cluster has exchanged the maxima and sums.
+#include <algorithm>
+#include <atomic>
+
 #include "ms_window.cuh"
 
 namespace ms {
 namespace {
 
-constexpr int kMaxGroup = 8;
+using namespace attn;
+
+constexpr int kMaxCluster = 16;
 
 struct RowsParams {
-  WindowArgs a;
-  int group;
-  float qscale;
+  const void *q, *k_pool, *v_pool;
+  const int32_t *block_tables, *row_table, *row_ctx;
+  void *out;
+  float *weight_sum, *raw;  // K3a: accumulators; raw scores [rows][Hkv][G][ctx16]
+  int64_t weight_stride;
   unsigned *status;
+  int pool_blocks, table_rows, max_blocks_per_seq;
+  int max_ctx, ctx16;
+  int window, sinks;
+  int num_kv_heads, group;
+  float qscale;  // softmax scale * log2(e)
+  int wait_limit;
 };
 
-template <typename T, int D>
-__global__ void __launch_bounds__(128) window_rows_kernel(RowsParams p) {
-  constexpr int DPL = D / 32, W = 4;
-  const WindowArgs &a = p.a;
-  const int kvh = blockIdx.y, G = p.group;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int row = blockIdx.x, ctx = a.row_ctx[row], trow = a.row_table ? a.row_table[row] : row;
-  bool ok = ctx >= 0 && ctx <= a.max_ctx;
-  ok = ok && trow >= 0 && trow < a.table_rows;
-  if (a.weight_sum && table_row_repeated(a.row_table, row, trow)) ok = false;
-  if (!ok) {
-    if (threadIdx.x == 0) atomicOr(p.status, kStatusBadIndex);
-    return;
-  }
-  const int32_t *table = a.block_tables + size_t(trow) * a.max_blocks_per_seq;
-  const int low = VisiblePages::lowest_key(ctx - 1, a.window);
-  const int nsink = min(a.sinks, low), nvis = nsink + ctx - low;
-  const T *q = static_cast<const T *>(a.q) + (size_t(row) * a.num_kv_heads + kvh) * G * D;
-  T *out = static_cast<T *>(a.out) + (size_t(row) * a.num_kv_heads + kvh) * G * D;
-  float *raw = a.weight_sum ? static_cast<float *>(a.workspace) + (size_t(row) * a.num_kv_heads + kvh) * G * a.max_ctx
-                            : nullptr;
+// bits 0 .. n - 1 set (none for n <= 0, all from n = 32 on)
+__device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : 0xffffffffu >> (32 - min(n, 32)); }
 
-  float qv[kMaxGroup][DPL], o[kMaxGroup][DPL], m[kMaxGroup], l[kMaxGroup];
+// ---- one page of one kv head: 16-bit K/V on mma.sync ----------------------------------
+template <typename T_, int D_, int NSTAGE_> struct PageTc {
+  using T = T_;
+  static constexpr int D = D_, NSTAGE = NSTAGE_;
+  static constexpr int NDH = D / 64, TILE_BYTES = NDH * kHalfBytes, KSTEPS = D / 16, NTD = D / 8;
+  uint32_t qa[KSTEPS][2];
+  float o[NTD][4];
+  float m_run = -INFINITY, l_run = 0.f;
+
+  __device__ __forceinline__ void init(const T *q, int group, float) {
+    const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
+    const T *row = q + (gid < group ? gid : 0) * D;
 #pragma unroll
-  for (int g = 0; g < kMaxGroup; ++g) {
-    m[g] = -INFINITY;
-    l[g] = 0.f;
+    for (int kk = 0; kk < KSTEPS; ++kk) {
+      qa[kk][0] = gid < group ? *reinterpret_cast<const uint32_t *>(row + kk * 16 + 2 * tig) : 0u;
+      qa[kk][1] = gid < group ? *reinterpret_cast<const uint32_t *>(row + kk * 16 + 8 + 2 * tig) : 0u;
+    }
 #pragma unroll
-    for (int d = 0; d < DPL; ++d) {
-      qv[g][d] = g < G ? Elem<T>::to_f(q[g * D + lane * DPL + d]) : 0.f;
-      o[g][d] = 0.f;
+    for (int nd = 0; nd < NTD; ++nd) o[nd][0] = o[nd][1] = o[nd][2] = o[nd][3] = 0.f;
+  }
+
+  static __device__ __forceinline__ void issue(unsigned char *st, const CUtensorMap &kmap, const CUtensorMap &vmap,
+                                               const RowsParams &, int page, int kvh, int hkv, uint64_t *bar) {
+    mbar_expect_tx(bar, 2 * TILE_BYTES);
+#pragma unroll
+    for (int dh = 0; dh < NDH; ++dh) {
+      tma_load_4d(st + dh * kHalfBytes, &kmap, 0, dh, 0, page * hkv + kvh, bar);
+      tma_load_4d(st + TILE_BYTES + dh * kHalfBytes, &vmap, 0, dh, 0, page * hkv + kvh, bar);
     }
   }
-  for (int i = warp; i < nvis; i += W) {
-    const int key = i < nsink ? i : low + i - nsink;
-    const int page = table[key / attn::kBS];
-    if (page < 0 || page >= a.pool_blocks) {
-      if (lane == 0) atomicOr(p.status, kStatusBadIndex);
-      continue;
+
+  // bits: visible tokens of the page, at least one.  raw: the page's scores of head 0, or null.
+  __device__ __forceinline__ void page(unsigned char *st, uint32_t bits, float qscale, float *raw, int raw_stride,
+                                       int group) {
+    const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3, mi = lane >> 3, lr = lane & 7;
+    const uint32_t kb = smem_addr(st), vb = kb + TILE_BYTES;
+    if (bits != 0xffffu) {
+      // what the row does not see may hold anything, NaN included: P = 0 must meet V = 0
+      uint4 *vz = reinterpret_cast<uint4 *>(st + TILE_BYTES);
+#pragma unroll
+      for (int i = lane; i < NDH * kBS * 8; i += 32)
+        if (!(bits >> ((i >> 3) & 15) & 1)) vz[i] = make_uint4(0u, 0u, 0u, 0u);
+      __syncwarp();
     }
-    const size_t at = ((size_t(page) * a.num_kv_heads + kvh) * attn::kBS + key % attn::kBS) * D + lane * DPL;
-    float k[DPL], v[DPL];
+    float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-    for (int d = 0; d < DPL; ++d) {
-      k[d] = Elem<T>::to_f(static_cast<const T *>(a.k_pool)[at + d]);
-      v[d] = Elem<T>::to_f(static_cast<const T *>(a.v_pool)[at + d]);
+    for (int kk = 0; kk < KSTEPS; ++kk) {
+      uint32_t b[4];
+      ldmatrix_x4(b, kb + tile_off((mi >> 1) * 8 + lr, kk * 16 + (mi & 1) * 8));
+      const uint32_t a[4] = {qa[kk][0], 0u, qa[kk][1], 0u};
+      mma_16816<T>(sc[0], a, b[0], b[1]);
+      mma_16816<T>(sc[1], a, b[2], b[3]);
     }
+    // row gid: tokens 2 tig, 2 tig + 1, 8 + 2 tig, 9 + 2 tig
+    float sv[4] = {sc[0][0], sc[0][1], sc[1][0], sc[1][1]};
+    float mx = -INFINITY;
 #pragma unroll
-    for (int g = 0; g < kMaxGroup; ++g) {
-      if (g >= G) break;
-      float s = 0.f;
+    for (int j = 0; j < 4; ++j) {
+      const int tk = 2 * tig + (j & 1) + 8 * (j >> 1);
+      sv[j] = bits >> tk & 1 ? sv[j] * qscale : -INFINITY;
+      mx = fmaxf(mx, sv[j]);
+    }
+    if (raw && gid < group) {  // (slots past the row's context: inside the 16-slot rounding)
+      float *r = raw + size_t(gid) * raw_stride;
+      *reinterpret_cast<float2 *>(r + 2 * tig) = make_float2(sv[0], sv[1]);
+      *reinterpret_cast<float2 *>(r + 8 + 2 * tig) = make_float2(sv[2], sv[3]);
+    }
+    mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 2));
+    const float m_new = fmaxf(m_run, mx);
+    const float alpha = exp2f(m_run - m_new);
+    float pj[4], psum = 0.f;
 #pragma unroll
-      for (int d = 0; d < DPL; ++d) s = fmaf(qv[g][d], k[d], s);
-      s = warp_sum(s) * p.qscale;
-      if (raw && lane == 0) raw[size_t(g) * a.max_ctx + key] = s;
-      const float mn = fmaxf(m[g], s), f = exp2f(m[g] - mn), e = exp2f(s - mn);
-      l[g] = l[g] * f + e;
-      m[g] = mn;
+    for (int j = 0; j < 4; ++j) {
+      pj[j] = exp2f(sv[j] - m_new);
+      psum += pj[j];
+    }
+    l_run = l_run * alpha + psum;
+    m_run = m_new;
 #pragma unroll
-      for (int d = 0; d < DPL; ++d) o[g][d] = fmaf(e, v[d], o[g][d] * f);
+    for (int nd = 0; nd < NTD; ++nd) {
+      o[nd][0] *= alpha;
+      o[nd][1] *= alpha;
+    }
+    // P is rounded to the K/V type for the tensor cores (the sum above is not): half a step
+    // relative per weight, which the result's own rounding matches
+    const uint32_t pa[4] = {pack2<T>(pj[0], pj[1]), 0u, pack2<T>(pj[2], pj[3]), 0u};
+#pragma unroll
+    for (int ndp = 0; ndp < NTD / 2; ++ndp) {
+      uint32_t b[4];
+      ldmatrix_x4_trans(b, vb + tile_off((mi & 1) * 8 + lr, (2 * ndp + (mi >> 1)) * 8));
+      mma_16816<T>(o[2 * ndp], pa, b[0], b[1]);
+      mma_16816<T>(o[2 * ndp + 1], pa, b[2], b[3]);
     }
   }
-  __shared__ float so[W][kMaxGroup][D], sm[W][kMaxGroup], sl[W][kMaxGroup];
+
+  // this warp's O [group][D], maxima and sums to shared memory
+  __device__ __forceinline__ void store(float *mo, float *mm, float *ml, int group) {
+    const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
+    l_run += __shfl_xor_sync(kFull, l_run, 1);
+    l_run += __shfl_xor_sync(kFull, l_run, 2);
+    if (gid >= group) return;
 #pragma unroll
-  for (int g = 0; g < kMaxGroup; ++g) {
+    for (int nd = 0; nd < NTD; ++nd)
+      *reinterpret_cast<float2 *>(mo + gid * D + nd * 8 + 2 * tig) = make_float2(o[nd][0], o[nd][1]);
+    if (tig == 0) {
+      mm[gid] = m_run;
+      ml[gid] = l_run;
+    }
+  }
+};
+
+// ---- one page of one kv head: f32 on the FMA pipe ---------------------------------------
+template <int D_, int G> struct PageF32 {
+  using T = float;
+  static constexpr int D = D_, NSTAGE = D == 128 ? 2 : 3;
+  static constexpr int DPL = D / 32, TILE = kBS * D, TILE_BYTES = TILE * 4;
+  static constexpr int SUB = (G > 4) ? 8 : 16;  // tokens per scoring sub-tile
+  static constexpr int NV = G * SUB, NVP = ((NV + 31) / 32) * 32;
+  static constexpr int R = NVP / 32;   // totals per lane after the butterfly
+  static constexpr int LPH = SUB / R;  // lanes per head
+  static_assert(LPH * R == SUB && LPH * G <= 32, "lane mapping");
+  float qv[G][DPL], acc[G][DPL], m_run[G];
+  float l_lane = 0.f;
+
+  __device__ __forceinline__ void init(const float *q, int, float qscale) {
+    const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int d = 0; d < DPL; ++d) so[warp][g][lane * DPL + d] = o[g][d];
-    if (lane == 0) {
-      sm[warp][g] = m[g];
-      sl[warp][g] = l[g];
+    for (int h = 0; h < G; ++h) {
+      TileLoad<float, D>::load(q + h * D, lane, qv[h]);
+      m_run[h] = -INFINITY;
+#pragma unroll
+      for (int d = 0; d < DPL; ++d) {
+        qv[h][d] *= qscale;
+        acc[h][d] = 0.f;
+      }
     }
   }
-  __syncthreads();
-  for (int i = threadIdx.x; i < G * D; i += 128) {
-    const int g = i / D, d = i % D;
-    float M = -INFINITY, L = 0.f, O = 0.f;
-    for (int w = 0; w < W; ++w) M = fmaxf(M, sm[w][g]);
-    for (int w = 0; w < W; ++w) {
-      const float f = sm[w][g] == -INFINITY ? 0.f : exp2f(sm[w][g] - M);
-      L += f * sl[w][g];
-      O += f * so[w][g][d];
-    }
-    out[i] = Elem<T>::from_f(L > 0.f ? O / L : 0.f);
+
+  static __device__ __forceinline__ void issue(unsigned char *st, const CUtensorMap &, const CUtensorMap &,
+                                               const RowsParams &p, int page, int kvh, int hkv, uint64_t *bar) {
+    const size_t at = (size_t(page) * hkv + kvh) * TILE;
+    mbar_expect_tx(bar, 2 * TILE_BYTES);
+    bulk_g2s(st, static_cast<const float *>(p.k_pool) + at, TILE_BYTES, bar);
+    bulk_g2s(st + TILE_BYTES, static_cast<const float *>(p.v_pool) + at, TILE_BYTES, bar);
   }
-  if (!raw) return;
-  float *sum = a.weight_sum + (size_t(trow) * a.num_kv_heads + kvh) * a.weight_stride;
-  for (int key = threadIdx.x; key < ctx; key += 128) {
-    const int page = table[key / attn::kBS];
-    if (page < 0 || page >= a.pool_blocks) continue;
-    float add = 0.f;
-    for (int g = 0; g < G; ++g) {
-      float M = -INFINITY, L = 0.f;
-      for (int w = 0; w < W; ++w) M = fmaxf(M, sm[w][g]);
-      for (int w = 0; w < W; ++w) L += sm[w][g] == -INFINITY ? 0.f : exp2f(sm[w][g] - M) * sl[w][g];
-      add += exp2f(raw[size_t(g) * a.max_ctx + key] - M) / L;
+
+  __device__ __forceinline__ void page(unsigned char *st, uint32_t bits, float, float *raw, int raw_stride, int) {
+    const int lane = threadIdx.x & 31;
+    const float *kt = reinterpret_cast<const float *>(st), *vt = kt + TILE;
+    const int hl = lane / LPH;  // head of this lane's score totals (>= G: padding lane)
+#pragma unroll
+    for (int t0 = 0; t0 < kBS; t0 += SUB) {
+      const uint32_t live = bits >> t0 & ((1u << SUB) - 1);  // warp-uniform
+      if (!live) {
+        if (raw && hl < G)
+#pragma unroll
+          for (int j = 0; j < R; ++j) raw[size_t(hl) * raw_stride + t0 + (lane * R + j) % SUB] = -INFINITY;
+        continue;
+      }
+      float v[NVP];
+#pragma unroll
+      for (int i = 0; i < NVP; ++i) v[i] = 0.f;
+#pragma unroll
+      for (int t = 0; t < SUB; ++t) {
+        if (live >> t & 1) {
+          float kk[DPL];
+          TileLoad<float, D>::load(kt + (t0 + t) * D, lane, kk);
+#pragma unroll
+          for (int h = 0; h < G; ++h) {
+            float a = 0.f;
+#pragma unroll
+            for (int d = 0; d < DPL; ++d) a = fmaf(qv[h][d], kk[d], a);
+            v[h * SUB + t] = a;
+          }
+        }
+      }
+      Butterfly<NVP, 16>::run(v, lane);
+      // lane holds totals for index lane * R + j -> head hl, token (lane * R + j) % SUB
+      float mloc = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < R; ++j) {
+        const int t = (lane * R + j) % SUB;
+        if (hl >= G || !(live >> t & 1)) v[j] = -INFINITY;
+        if (raw && hl < G) raw[size_t(hl) * raw_stride + t0 + t] = v[j];
+        mloc = fmaxf(mloc, v[j]);
+      }
+#pragma unroll
+      for (int o = LPH / 2; o > 0; o >>= 1) mloc = fmaxf(mloc, __shfl_xor_sync(kFull, mloc, o));
+      float alpha[G], mh = -INFINITY, al = 1.f;
+#pragma unroll
+      for (int h = 0; h < G; ++h) {
+        const float mn = fmaxf(m_run[h], __shfl_sync(kFull, mloc, h * LPH));
+        alpha[h] = exp2f(m_run[h] - mn);
+        m_run[h] = mn;
+        if (hl == h) {
+          mh = mn;
+          al = alpha[h];
+        }
+      }
+      float pv[R], psum = 0.f;
+#pragma unroll
+      for (int j = 0; j < R; ++j) {
+        pv[j] = (v[j] == -INFINITY) ? 0.f : exp2f(v[j] - mh);
+        psum += pv[j];
+      }
+      l_lane = l_lane * al + psum;
+#pragma unroll
+      for (int h = 0; h < G; ++h)
+#pragma unroll
+        for (int d = 0; d < DPL; ++d) acc[h][d] *= alpha[h];
+#pragma unroll
+      for (int t = 0; t < SUB; ++t) {
+        if (live >> t & 1) {
+          float vv[DPL];
+          TileLoad<float, D>::load(vt + (t0 + t) * D, lane, vv);
+#pragma unroll
+          for (int h = 0; h < G; ++h) {
+            const int idx = h * SUB + t;
+            const float ph = __shfl_sync(kFull, pv[idx % R], idx / R);
+#pragma unroll
+            for (int d = 0; d < DPL; ++d) acc[h][d] = fmaf(ph, vv[d], acc[h][d]);
+          }
+        }
+      }
     }
-    sum[key] += add;
   }
+
+  __device__ __forceinline__ void store(float *mo, float *mm, float *ml, int) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = LPH / 2; o > 0; o >>= 1) l_lane += __shfl_xor_sync(kFull, l_lane, o);
+#pragma unroll
+    for (int h = 0; h < G; ++h) {
+#pragma unroll
+      for (int d = 0; d < DPL; ++d) mo[h * D + lane * DPL + d] = acc[h][d];
+      const float lh = __shfl_sync(kFull, l_lane, h * LPH);
+      if (lane == 0) {
+        mm[h] = m_run[h];
+        ml[h] = lh;
+      }
+    }
+  }
+};
+
+// ---- clusters ------------------------------------------------------------------------------
+__device__ __forceinline__ void cluster_arrive() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// the f32 / i32 at `p` (this CTA's shared memory) in CTA `rank` of the cluster
+__device__ __forceinline__ float peer_f32(const float *p, int rank) {
+  uint32_t a;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
 }
 
-template <typename T>
-cudaError_t launch_rows(const RowsParams &p, cudaStream_t stream) {
-  const dim3 grid(p.a.num_rows, p.a.num_kv_heads);
-  if (p.a.head_dim == 128) window_rows_kernel<T, 128><<<grid, 128, 0, stream>>>(p);
-  else window_rows_kernel<T, 64><<<grid, 128, 0, stream>>>(p);
-  return cudaGetLastError();
+constexpr int kMaxGroup = 8;
+
+// Page::D * kMaxGroup floats for each warp's O and the CTA's; the maxima and sums of both
+template <class Page> struct Layout {
+  static constexpr size_t kStages = size_t(kWarps) * Page::NSTAGE * 2 * Page::TILE_BYTES;
+  static constexpr size_t kBars = kWarps * Page::NSTAGE * sizeof(uint64_t);
+  static constexpr size_t kMerge = (size_t(kWarps) + 1) * kMaxGroup * (Page::D + 2) * sizeof(float);
+  static constexpr size_t kSmem = 1024 + std::max(kStages + kBars, kMerge);
+};
+
+template <class Page, bool WEIGHTS>
+__global__ void __launch_bounds__(kWarps * 32)
+    window_rows_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                       RowsParams p, int C) {
+  constexpr int NSTAGE = Page::NSTAGE, STAGE_BYTES = 2 * Page::TILE_BYTES, D = Page::D;
+  using T = typename Page::T;
+  extern __shared__ unsigned char smem_dyn[];
+  unsigned char *smem =
+      reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + Layout<Page>::kStages);
+
+  const int row = blockIdx.x / C, part = blockIdx.x % C;  // part = rank in the cluster
+  const int kvh = blockIdx.y, G = p.group;
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+  const int ctx = p.row_ctx[row], trow = p.row_table ? p.row_table[row] : row;
+  bool ok = ctx >= 0 && ctx <= p.max_ctx && trow >= 0 && trow < p.table_rows;
+  if (WEIGHTS && table_row_repeated(p.row_table, row, trow)) ok = false;
+  if (!ok) {  // the whole cluster leaves
+    if (t == 0) atomicOr(p.status, kStatusBadIndex);
+    return;
+  }
+  const int32_t *table = p.block_tables + size_t(trow) * p.max_blocks_per_seq;
+  const int low = VisiblePages::lowest_key(ctx - 1, p.window);
+  const VisiblePages vis(ctx - 1, ctx, p.window, p.sinks);
+  const int share = (vis.count + C - 1) / C;
+  const int b0 = min(part * share, vis.count), b1 = min(b0 + share, vis.count);
+  const int nb_w = (b1 - b0 - warp + kWarps - 1) / kWarps;  // pages b0 + warp + k * kWarps
+  unsigned char *my_stage = smem + size_t(warp) * NSTAGE * STAGE_BYTES;
+  uint64_t *my_bar = bars + warp * NSTAGE;
+  if (lane == 0) {
+    for (int s = 0; s < NSTAGE; ++s) mbar_init(&my_bar[s], 1);
+    fence_barrier_init();
+    fence_proxy_async();
+  }
+  __syncwarp();
+
+  int page_reg = 0;  // lane k holds the page id of this warp's k-th page (32 at a time)
+  auto page_of = [&](int k) -> int { return __shfl_sync(kFull, page_reg, k & 31); };
+  auto refill_pages = [&](int k0) {
+    const int k = k0 + lane;
+    page_reg = 0;
+    if (k < nb_w) {
+      const int page = table[vis.page_at(b0 + warp + k * kWarps)];
+      if (page >= 0 && page < p.pool_blocks) page_reg = page;
+      else atomicOr(p.status, kStatusBadIndex);
+    }
+  };
+  auto issue = [&](int s, int page) {
+    if (lane == 0)
+      Page::issue(my_stage + size_t(s) * STAGE_BYTES, kmap, vmap, p, page, kvh, p.num_kv_heads, &my_bar[s]);
+  };
+  bool failed = false;
+  int issued = 0, kfail = 0;
+  if (nb_w > 0) {
+    refill_pages(0);
+    const int pro = min(NSTAGE, nb_w);
+    for (int k = 0; k < pro; ++k) issue(k, page_of(k));
+    issued = pro;
+  }
+  Page pg;
+  const size_t head0 = (size_t(row) * p.num_kv_heads + kvh) * G;
+  pg.init(static_cast<const T *>(p.q) + head0 * D, G, p.qscale);
+  float *raw = WEIGHTS ? p.raw + head0 * p.ctx16 : nullptr;
+
+  for (int k = 0; k < nb_w; ++k) {
+    const int s = k % NSTAGE;
+    // the whole warp agrees before leaving, so no lane is left waiting in a shuffle
+    if (!__all_sync(kFull, mbar_wait_bounded(&my_bar[s], (k / NSTAGE) & 1, p.wait_limit))) {
+      failed = true;
+      kfail = k;
+      break;
+    }
+    const int key0 = vis.page_at(b0 + warp + k * kWarps) * kBS;
+    const uint32_t bits =
+        0xffffu & bits_below(ctx - key0) & (~bits_below(low - key0) | bits_below(p.sinks - key0));
+    pg.page(my_stage + size_t(s) * STAGE_BYTES, bits, p.qscale, WEIGHTS ? raw + key0 : nullptr, p.ctx16, G);
+    __syncwarp();
+    if (issued < nb_w && k + NSTAGE == issued) {
+      const int kn = issued;
+      if ((kn & 31) == 0) refill_pages(kn);
+      const int page = page_of(kn);
+      if (lane == 0) fence_proxy_async();
+      issue(s, page);
+      ++issued;
+    }
+  }
+  if (failed) {
+    if (lane == 0) atomicOr(p.status, kStatusWaitTimeout);
+    for (int k = kfail; k < issued; ++k) mbar_wait_bounded(&my_bar[k % NSTAGE], (k / NSTAGE) & 1);
+  }
+
+  // ---- merge the warps (the stages are free), then the cluster's CTAs ----
+  float *wo = reinterpret_cast<float *>(smem);         // [kWarps][G][D]
+  float *wm = wo + kWarps * kMaxGroup * D;             // [kWarps][kMaxGroup] maxima, then sums
+  float *wl = wm + kWarps * kMaxGroup;
+  float *co = wl + kWarps * kMaxGroup;                 // the CTA's [G][D], maxima, sums
+  float *cm = co + kMaxGroup * D, *cl = cm + kMaxGroup;
+  const bool any_failed = __syncthreads_or(failed ? 1 : 0) != 0;
+  pg.store(wo + warp * kMaxGroup * D, wm + warp * kMaxGroup, wl + warp * kMaxGroup, G);
+  __syncthreads();
+  T *out = static_cast<T *>(p.out) + head0 * D;
+  for (int i = t; i < G * D; i += kWarps * 32) {
+    const int h = i / D;
+    float M = -INFINITY, L = 0.f, O = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) M = fmaxf(M, wm[w * kMaxGroup + h]);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float mw = wm[w * kMaxGroup + h], f = mw == -INFINITY ? 0.f : exp2f(mw - M);
+      L += f * wl[w * kMaxGroup + h];
+      O += f * wo[w * kMaxGroup * D + i];
+    }
+    if (C == 1 && !any_failed) out[i] = Elem<T>::from_f(L > 0.f ? O / L : 0.f);
+    co[i] = O;
+    if (i % D == 0) {
+      cm[h] = any_failed ? NAN : M;  // a NaN maximum tells the cluster that a wait ran out
+      cl[h] = L;
+    }
+  }
+  if (C > 1) {
+    cluster_arrive();
+    cluster_wait();
+    for (int i = part * kWarps * 32 + t; i < G * D; i += C * kWarps * 32) {
+      const int h = i / D;
+      float M = -INFINITY, L = 0.f, O = 0.f;
+      bool bad = false;
+      for (int c = 0; c < C; ++c) {
+        const float mc = peer_f32(cm + h, c);
+        bad |= mc != mc;
+        M = fmaxf(M, mc);
+      }
+      for (int c = 0; c < C; ++c) {
+        const float mc = peer_f32(cm + h, c), f = mc == -INFINITY ? 0.f : exp2f(mc - M);
+        L += f * peer_f32(cl + h, c);
+        O += f * peer_f32(co + i, c);
+      }
+      if (!bad) out[i] = Elem<T>::from_f(L > 0.f ? O / L : 0.f);
+    }
+  }
+  if constexpr (WEIGHTS) {
+    __syncthreads();
+    if (t < G) {  // the row's maximum and reciprocal sum (the warps' slots are free)
+      float M = -INFINITY, L = 0.f;
+      bool bad = false;
+      for (int c = 0; c < C; ++c) {
+        const float mc = C > 1 ? peer_f32(cm + t, c) : cm[t];
+        bad |= mc != mc;
+        M = fmaxf(M, mc);
+      }
+      for (int c = 0; c < C; ++c) {
+        const float mc = C > 1 ? peer_f32(cm + t, c) : cm[t];
+        L += mc == -INFINITY ? 0.f : exp2f(mc - M) * (C > 1 ? peer_f32(cl + t, c) : cl[t]);
+      }
+      wm[t] = bad ? NAN : M;
+      wl[t] = L > 0.f ? 1.f / L : 0.f;
+    }
+    __syncthreads();
+    if (C > 1) cluster_arrive();
+    float *sum = p.weight_sum + (size_t(trow) * p.num_kv_heads + kvh) * p.weight_stride;
+    if (wm[0] == wm[0])
+      for (int key = b0 * kBS + t; key < min(b1 * kBS, ctx); key += kWarps * 32) {
+        float add = 0.f;
+        for (int h = 0; h < G; ++h) add += exp2f(raw[size_t(h) * p.ctx16 + key] - wm[h]) * wl[h];
+        sum[key] += add;
+      }
+  } else {
+    if (C > 1) cluster_arrive();
+  }
+  if (C > 1) cluster_wait();  // no CTA leaves while another may read its shared memory
+}
+
+// CTAs per (row, kv head).  A CTA keeps 96 KB of copies in flight and two fit an SM, so the
+// machine is full from 2 x 148 CTAs on; fewer (row, kv head) pairs than that are split, down to
+// two pages a warp and to the 16 CTAs that a cluster holds.
+int cluster_size(int rows, int hkv, int max_pages) {
+  int c = 1;
+  while (c < kMaxCluster && (long long)rows * hkv * c < 2 * 148 && max_pages > 2 * kWarps * c) c *= 2;
+  return c;
+}
+
+template <class Page, bool WEIGHTS>
+cudaError_t launch_rows(const RowsParams &p, int rows, int C, const CUtensorMap &km, const CUtensorMap &vm,
+                        cudaStream_t stream) {
+  auto kern = window_rows_kernel<Page, WEIGHTS>;
+  static std::atomic<bool> attr_done[64];  // per device; zero-initialised (static storage)
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !attr_done[dev].load(std::memory_order_acquire)) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Layout<Page>::kSmem));
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64) attr_done[dev].store(true, std::memory_order_release);  // setting twice is harmless
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(rows) * C, p.num_kv_heads);
+  cfg.blockDim = dim3(kWarps * 32);
+  cfg.dynamicSmemBytes = Layout<Page>::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = C;
+  at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = C > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kern, km, vm, p, C);
+}
+
+template <class Page>
+cudaError_t launch_page(const RowsParams &p, int rows, int C, const CUtensorMap &km, const CUtensorMap &vm,
+                        cudaStream_t stream) {
+  return p.weight_sum ? launch_rows<Page, true>(p, rows, C, km, vm, stream)
+                      : launch_rows<Page, false>(p, rows, C, km, vm, stream);
+}
+
+template <int D>
+cudaError_t launch_f32(const RowsParams &p, int rows, int C, cudaStream_t stream) {
+  const CUtensorMap none{};
+  switch (p.group) {
+    case 1: return launch_page<PageF32<D, 1>>(p, rows, C, none, none, stream);
+    case 2: return launch_page<PageF32<D, 2>>(p, rows, C, none, none, stream);
+    case 4: return launch_page<PageF32<D, 4>>(p, rows, C, none, none, stream);
+    case 7: return launch_page<PageF32<D, 7>>(p, rows, C, none, none, stream);
+    case 8: return launch_page<PageF32<D, 8>>(p, rows, C, none, none, stream);
+    default: return cudaErrorInvalidValue;
+  }
 }
 
 cudaError_t launch_checked(const WindowArgs &a, cudaStream_t stream) {
   RowsParams p{};
-  p.a = a;
+  p.q = a.q;
+  p.k_pool = a.k_pool;
+  p.v_pool = a.v_pool;
+  p.block_tables = a.block_tables;
+  p.row_table = a.row_table;
+  p.row_ctx = a.row_ctx;
+  p.out = a.out;
+  p.weight_sum = a.weight_sum;
+  p.raw = static_cast<float *>(a.workspace);
+  p.weight_stride = a.weight_stride;
+  p.pool_blocks = int(a.pool_blocks);  // < 2^31 (pools_ok)
+  p.table_rows = a.table_rows;
+  p.max_blocks_per_seq = a.max_blocks_per_seq;
+  p.max_ctx = a.max_ctx;
+  p.ctx16 = (a.max_ctx + kBS - 1) / kBS * kBS;
+  p.window = a.window;
+  p.sinks = a.sinks;
+  p.num_kv_heads = a.num_kv_heads;
   p.group = a.num_heads / a.num_kv_heads;
-  p.qscale = a.scale * attn::kLog2e;
+  p.qscale = a.scale * kLog2e;
+  p.wait_limit = page_wait_limit();
   p.status = a.status;
   if (!p.status) {
     const cudaError_t e = standalone_status_word(&p.status);
     if (e != cudaSuccess) return e;
   }
-  if (a.dtype == MS_DTYPE_F32) return launch_rows<float>(p, stream);
-  if (a.dtype == MS_DTYPE_BF16) return launch_rows<__nv_bfloat16>(p, stream);
-  return launch_rows<__half>(p, stream);
+  // by the window where there is one, not by this call's contexts: a row's result does not
+  // change with the longest context it is batched with
+  const int64_t most = a.window > 0 ? int64_t(a.window) + a.sinks : a.max_ctx;
+  const int C = cluster_size(a.num_rows, a.num_kv_heads, int(std::min<int64_t>(most / kBS + 2, 1 << 26)));
+  if ((long long)a.num_rows * C > 0x7fffffffLL) return cudaErrorInvalidValue;
+  if (a.dtype == MS_DTYPE_F32)
+    return a.head_dim == 128 ? launch_f32<128>(p, a.num_rows, C, stream) : launch_f32<64>(p, a.num_rows, C, stream);
+  CUtensorMap km, vm;
+  const int64_t tiles = a.pool_blocks * a.num_kv_heads;
+  if (!encode_pool_tensor_map(&km, a.k_pool, a.dtype, a.head_dim, tiles) ||
+      !encode_pool_tensor_map(&vm, a.v_pool, a.dtype, a.head_dim, tiles))
+    return cudaErrorInvalidValue;
+  if (a.dtype == MS_DTYPE_BF16)
+    return a.head_dim == 128 ? launch_page<PageTc<__nv_bfloat16, 128, 3>>(p, a.num_rows, C, km, vm, stream)
+                             : launch_page<PageTc<__nv_bfloat16, 64, 4>>(p, a.num_rows, C, km, vm, stream);
+  return a.head_dim == 128 ? launch_page<PageTc<__half, 128, 3>>(p, a.num_rows, C, km, vm, stream)
+                           : launch_page<PageTc<__half, 64, 4>>(p, a.num_rows, C, km, vm, stream);
 }
 
 bool common_ok(const WindowArgs &a) {

@@ -406,3 +406,28 @@ def test_streams_and_graph_replay():
     assert all(torch.equal(o[n], again[n]) for n in ("row", "chunk", "wrow", "w"))
     assert not torch.equal(o["row"], want["row"])
     assert E.kernel_status(0) == 0
+
+
+def test_a_wait_that_runs_out_is_reported():
+    """The poll limit set to zero: no copy has landed at the first poll, every
+    one still lands before the CTA leaves; nothing is written, the status says so."""
+    lib = E.lib()
+    hkv, d, dt = 2, 128, torch.bfloat16
+    for rows in (1, 200):  # split over a cluster, and not
+        ctx = [3000] * rows
+        g = torch.Generator().manual_seed(0)
+        k, v = (torch.randn(400, hkv, 16, d, generator=g).to(dt).to(DEV) for _ in range(2))
+        tables = torch.randint(0, 400, (rows, 188), generator=g).to(torch.int32).to(DEV)
+        q = torch.randn(rows, 4, d, generator=g).to(dt).to(DEV)
+        rt = torch.arange(rows, dtype=torch.int32, device=DEV)
+        good, out, w = torch.full_like(q, 5.0), torch.full_like(q, 5.0), torch.zeros(rows, hkv, 3000, device=DEV)
+        try:
+            lib.ms_test_set_attention_wait_limit(0)
+            sync_ok(run_rows(q, k, v, tables, rt, ctx, 2000, 4, out))
+            assert E.kernel_status(0) == 1 and (out == 5.0).all()
+            sync_ok(run_weights(q, k, v, tables, rt, ctx, out, w))
+            assert E.kernel_status(0) == 1 and (out == 5.0).all() and (w == 0).all()
+        finally:
+            lib.ms_test_set_attention_wait_limit(-1)
+        sync_ok(run_rows(q, k, v, tables, rt, ctx, 2000, 4, good))
+        assert E.kernel_status(0) == 0 and not (good == 5.0).any()
