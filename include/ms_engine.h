@@ -490,7 +490,7 @@ int ms_launch_attention_weights(const void *q, const void *k_pool, const void *v
  *    positions, weight_out[keep, n) zeros; the rest is left as it was.
  *    weight_out may be weight_in and pos_out may be pos_in.
  * weight_* f32 and pos_* int32 [table_rows, num_kv_heads, stride], stride >=
- * max_ctx, max_ctx <= 49152.  A table row may appear once per call, and the
+ * max_ctx, max_ctx <= 262144.  A table row may appear once per call, and the
  * listed sequences must own their pages: a page two of them share (a cached
  * prefix) would be overwritten for both.  workspace:
  * ms_evict_workspace_bytes. */

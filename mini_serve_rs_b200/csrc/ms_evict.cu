@@ -8,18 +8,40 @@
 // never a source, so the copies are independent of one another and only what
 // has to move moves; attention does not depend on the order of its keys.
 //
-// One CTA per (sequence, kv head).  The rank of a slot is a 32-bit key whose
-// unsigned order is the order of the weights (protected slots: the largest
-// key).  The keep-th largest key T is found bit by bit: 32 counts of the keys
-// >= a candidate, held in shared memory.  Slots above T stay, and of the slots
-// equal to T the lowest ones that still fit.
+// Two launches.  The first selects: a cluster of C CTAs serves one (sequence, kv
+// head); each holds a run of slots, their 32-bit rank keys (whose unsigned order
+// is the order of the weights; protected slots: the largest key) in shared
+// memory.
+//  1. T, the keep-th largest key, by a radix search of three digits from the
+//     top (11, 11 and 10 bits): histogram of the keys that match the digits
+//     found so far, summed over the cluster through distributed shared memory,
+//     and the digit in which the keep-th largest lies.  It ends early where
+//     all keys with T's digits so far stay.
+//  2. Slots above T stay, and of the slots equal to T the lowest that still
+//     fit: one bit each.  Counts of holes and movers per word, scanned over the
+//     CTA and the cluster, give each its rank; the lists of holes and movers
+//     and their length go to the workspace.
+// The second moves: 8 moves a warp (256-byte rows), all of a call's moves at
+// once on as many warps, because a row in a large pool costs a long latency
+// (address translation included) and few bytes: with the moves left to the CTA
+// that selected them, 8 at a time per warp, the longest sequences of a ragged
+// batch finished long after the others (64 sequences: 68 us against 33).
+// Latency-bound for one sequence (a chain of loads and barriers), bound by the
+// moves' HBM traffic for many.
+#include <algorithm>
+#include <atomic>
+
 #include "ms_window.cuh"
 
 namespace ms {
 namespace {
 
-constexpr int kThreads = 1024;
-constexpr int kMaxSlots = 49152;  // keys of one CTA in shared memory
+using attn::kBS;
+
+constexpr int kMaxCluster = 8;
+constexpr int kMaxSlots = 32768;  // rank keys of one CTA in shared memory
+constexpr int kDigits = 3;
+constexpr int kBins = 2048;
 
 struct EvictParams {
   unsigned char *k_pool, *v_pool;
@@ -27,15 +49,17 @@ struct EvictParams {
   const int32_t *block_tables;
   int table_rows, max_blocks_per_seq;
   const int32_t *row_table, *row_ctx, *row_next, *row_known;
-  int num_rows, max_ctx, keep, sinks, recent;
+  int max_ctx, keep, sinks, recent;
   const float *w_in;
   float *w_out;
   const int32_t *pos_in;
   int32_t *pos_out;
   int64_t stride;
   int num_kv_heads;
-  int row_bytes;  // head_dim * element size
-  int32_t *lists;  // [rows][kv heads][2][max_ctx]: holes, movers
+  int chunks;      // 16-byte pieces of one K (V) row
+  int32_t *lists;  // [rows][kv heads][2][half]: holes, movers
+  int half;
+  int32_t *moves;  // [rows][kv heads]: their number
   unsigned *status;
 };
 
@@ -46,38 +70,120 @@ __device__ __forceinline__ uint32_t rank_key(float w) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-__device__ __forceinline__ int block_count(int v, int *part) {
-  v = __reduce_add_sync(kFull, v);
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
-  __syncthreads();
-  const int t = __reduce_add_sync(kFull, part[threadIdx.x & 31]);
-  __syncthreads();
-  return t;
-}
+struct Shared {
+  uint32_t hist[kDigits][kBins];  // of each digit (read by the cluster)
+  uint32_t slice[kBins / 2];      // the cluster's sum of the bins this CTA adds up (read by the cluster)
+  uint32_t warp_sum[32];
+  uint32_t counts[2];             // this CTA's equal slots; holes | movers << 16 (read by the cluster)
+  uint32_t digit;
+  int left, equal;
+};
 
-// number of set flags in the threads before this one; total over the CTA in `total`
-__device__ __forceinline__ int block_rank(bool flag, int *part, int &total) {
-  const unsigned b = __ballot_sync(kFull, flag);
+// sum of v over the threads before this one; the CTA's total in `all`.  `scratch` is free again
+// after the next barrier.
+template <int NT>
+__device__ __forceinline__ uint32_t scan_before(uint32_t v, uint32_t *scratch, uint32_t &all) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (lane == 0) part[warp] = __popc(b);
+  uint32_t s = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t u = __shfl_up_sync(kFull, s, o);
+    if (lane >= o) s += u;
+  }
+  if (lane == 31) scratch[warp] = s;
   __syncthreads();
-  const int c = part[lane];
-  const int before = __reduce_add_sync(kFull, lane < warp ? c : 0);
-  total = __reduce_add_sync(kFull, c);
-  __syncthreads();
-  return before + __popc(b & ((1u << lane) - 1));
+  const uint32_t c = lane < NT / 32 ? scratch[lane] : 0;
+  all = __reduce_add_sync(kFull, c);
+  return __reduce_add_sync(kFull, lane < warp ? c : 0u) + s - v;
 }
 
-__global__ void __launch_bounds__(kThreads) evict_kernel(EvictParams p) {
+// The digit in which the keep-th largest value lies, counted from the top, over the cluster's
+// histograms of digit d (complete in shared memory): into sh.digit, sh.left (what is left to
+// find inside it) and sh.equal (the values in it), behind a barrier.
+template <int NT>
+__device__ __forceinline__ void find_digit(Shared &sh, int d, int C, int keep) {
+  constexpr int B = kBins / NT;  // bins of a thread, the largest digits first
+  const int t = threadIdx.x, b0 = kBins - B * (t + 1);
+  uint32_t c[B];
+  // CTA r adds up the r-th of C slices of the bins, then everyone takes the sums from their
+  // owners: 2 x 8 KB of distributed shared memory per CTA instead of C x 8 KB
+  const int slice = kBins / C;
+  if (C > 1) {
+    const int own = int(blockIdx.x % C) * slice;
+    for (int i = 4 * t; i < slice; i += 4 * NT) {
+      uint4 v = make_uint4(0, 0, 0, 0);
+      for (int r = 0; r < C; ++r) {
+        const uint4 u = peer_u4(&sh.hist[d][own + i], r);
+        v.x += u.x;
+        v.y += u.y;
+        v.z += u.z;
+        v.w += u.w;
+      }
+      *reinterpret_cast<uint4 *>(&sh.slice[i]) = v;
+    }
+    cluster_sync();
+  }
+#pragma unroll
+  for (int i = 0; i < B; i += 4) {
+    const int b = b0 + i;
+    const uint4 v = C == 1 ? *reinterpret_cast<const uint4 *>(&sh.hist[d][b]) : peer_u4(&sh.slice[b % slice], b / slice);
+    c[i] = v.x;
+    c[i + 1] = v.y;
+    c[i + 2] = v.z;
+    c[i + 3] = v.w;
+  }
+  uint32_t sum = 0, all;
+#pragma unroll
+  for (int i = 0; i < B; ++i) sum += c[i];
+  uint32_t above = scan_before<NT>(sum, sh.warp_sum, all);
+  if (above < uint32_t(keep) && above + sum >= uint32_t(keep)) {  // one thread
+#pragma unroll
+    for (int i = B - 1; i >= 0; --i) {
+      if (above < uint32_t(keep) && above + c[i] >= uint32_t(keep)) {
+        sh.digit = b0 + i;
+        sh.left = keep - int(above);
+        sh.equal = int(c[i]);
+      }
+      above += c[i];
+    }
+  }
+  __syncthreads();
+}
+
+// the n lowest set bits of w
+__device__ __forceinline__ uint32_t lowest_bits(uint32_t w, int n) {
+  if (n >= __popc(w)) return w;
+  uint32_t out = 0;
+  for (; n > 0; --n) {
+    out |= w & (0u - w);
+    w &= w - 1;
+  }
+  return out;
+}
+
+template <int NT>
+__global__ void __launch_bounds__(NT, 1024 / NT) evict_kernel(EvictParams p, int C, int seg) {
+  constexpr int kWarpsNT = NT / 32;
+  // [seg] rank keys, then [seg / 32] words three times
   extern __shared__ uint32_t keys[];
-  __shared__ int part[32];
-  const int row = blockIdx.x, h = blockIdx.y, t = threadIdx.x;
+  uint32_t *stay = keys + seg;        // slots above T, then slots that stay, one bit each
+  uint32_t *equal_w = stay + seg / 32;  // slots equal to T, then movers before each word
+  uint32_t *hole0 = equal_w + seg / 32;  // holes before each word
+  __shared__ Shared sh;
+  const int row = blockIdx.x / C, part = blockIdx.x % C, h = blockIdx.y;
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
   const int n = p.row_ctx[row], next = p.row_next[row], trow = p.row_table ? p.row_table[row] : row;
   const int known = p.row_known ? p.row_known[row] : 0;
+  for (int i = t; i < kDigits * kBins / 4; i += NT)
+    reinterpret_cast<uint4 *>(sh.hist)[i] = make_uint4(0, 0, 0, 0);
   bool ok = n >= 0 && n <= p.max_ctx && trow >= 0 && trow < p.table_rows && known >= 0 && next >= n;
-  if (table_row_repeated(p.row_table, row, trow)) ok = false;
-  if (!ok) {
-    if (t == 0) atomicOr(p.status, kStatusBadIndex);
+  if (table_row_repeated(p.row_table, row, trow)) ok = false;  // (with a barrier)
+  const size_t pair = size_t(row) * p.num_kv_heads + h;
+  if (!ok) {  // the whole cluster leaves
+    if (t == 0) {
+      atomicOr(p.status, kStatusBadIndex);
+      if (part == 0) p.moves[pair] = 0;
+    }
     return;
   }
   const size_t base = (size_t(trow) * p.num_kv_heads + h) * size_t(p.stride);
@@ -86,80 +192,244 @@ __global__ void __launch_bounds__(kThreads) evict_kernel(EvictParams p) {
   const int32_t *pos_in = p.pos_in ? p.pos_in + base : nullptr;
   int32_t *pos_out = p.pos_out + base;
   auto position = [&](int j) { return j < known ? pos_in[j] : next - n + j; };
+  const int s0 = part * seg, s1 = min(s0 + seg, n), len = max(0, s1 - s0);  // this CTA's slots
   if (n <= p.keep) {  // nothing to evict
-    for (int j = t; j < n; j += kThreads) {
+    if (part == 0 && t == 0) p.moves[pair] = 0;
+    for (int j = s0 + t; j < s1; j += NT) {
       w_out[j] = w_in[j];
       pos_out[j] = position(j);
     }
     return;
   }
-  for (int j = t; j < n; j += kThreads) {
-    const int pos = position(j);
-    keys[j] = pos < p.sinks || pos >= next - p.recent ? 0xffffffffu : rank_key(w_in[j]);
-  }
-  __syncthreads();
-  // T = the largest value that at least keep keys reach
-  uint32_t T = 0;
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t c = T | (1u << bit);
-    int v = 0;
-    for (int j = t; j < n; j += kThreads) v += keys[j] >= c;
-    if (block_count(v, part) >= p.keep) T = c;
-  }
-  int above = 0;
-  for (int j = t; j < n; j += kThreads) above += keys[j] > T;
-  const int ties = p.keep - block_count(above, part);  // slots equal to T that stay
 
-  int32_t *holes = p.lists + (size_t(row) * p.num_kv_heads + h) * 2 * size_t(p.max_ctx), *movers = holes + p.max_ctx;
-  int seen = 0, nh = 0, nm = 0;  // equal slots, holes, movers so far
-  for (int j0 = 0; j0 < n; j0 += kThreads) {
-    const int j = j0 + t;
-    const uint32_t key = j < n ? keys[j] : 0;
-    int total;
-    const int tie = seen + block_rank(j < n && key == T, part, total);
-    seen += total;
-    const bool kept = j < n && (key > T || (key == T && tie < ties));
-    const bool hole = j < p.keep && !kept, mover = j >= p.keep && kept;
-    const int ih = nh + block_rank(hole, part, total);
-    nh += total;
-    if (hole) holes[ih] = j;
-    const int im = nm + block_rank(mover, part, total);
-    nm += total;
-    if (mover) movers[im] = j;
-    if (j < p.keep && kept) {
-      w_out[j] = w_in[j];
-      pos_out[j] = position(j);
+  // ---- 1. the keep-th largest key ----
+  constexpr int U = 8;  // loads of U slots per thread before the first is used
+  for (int j0 = s0 + t; j0 < s1; j0 += U * NT) {
+    float w[U];
+    int pos[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = j0 + u * NT;
+      w[u] = j < s1 ? w_in[j] : 0.f;
+      pos[u] = j < s1 ? position(j) : 0;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = j0 + u * NT;
+      if (j < s1) {
+        const uint32_t key = pos[u] < p.sinks || pos[u] >= next - p.recent ? 0xffffffffu : rank_key(w[u]);
+        keys[j - s0] = key;
+        atomicAdd(&sh.hist[0][key >> 21], 1u);
+      }
+    }
+  }
+  uint32_t T = 0;
+  int left = p.keep, equal = 0;  // of the keys with T's digits so far: to keep, and in all
+#pragma unroll
+  for (int d = 0; d < kDigits; ++d) {
+    const int shift = d == 0 ? 21 : d == 1 ? 10 : 0;
+    if (d > 0) {
+      const int up = d == 1 ? 21 : 10;
+      const uint32_t mask = d == 1 ? 2047u : 1023u;
+#pragma unroll 4
+      for (int j = t; j < len; j += NT) {
+        const uint32_t key = keys[j];
+        if (key >> up == T >> up) atomicAdd(&sh.hist[d][key >> shift & mask], 1u);
+      }
+    }
+    if (C > 1) cluster_sync();
+    else __syncthreads();
+    find_digit<NT>(sh, d, C, left);
+    T |= sh.digit << shift;
+    left = sh.left;
+    equal = sh.equal;
+    if (left == equal) break;  // all of them stay: T's other digits may be 0 (the same for the cluster)
+  }
+
+  // ---- 2. which slots stay; holes and movers in order ----
+  const bool all_equal = left == equal;  // key >= T stays; else key > T, and the lowest `left` equal ones
+  const int words = (len + 31) / 32;
+  for (int i = warp; i < words; i += kWarpsNT) {
+    const int j = i * 32 + lane;
+    const uint32_t key = j < len ? keys[j] : 0u;
+    const unsigned gt = __ballot_sync(kFull, j < len && (all_equal ? key >= T : key > T));
+    const unsigned eq = __ballot_sync(kFull, j < len && key == T);
+    if (lane == 0) {
+      stay[i] = gt;
+      equal_w[i] = eq;
     }
   }
   __syncthreads();
-  const int32_t *table = p.block_tables + size_t(trow) * p.max_blocks_per_seq;
-  const int chunks = p.row_bytes / 16;
-  for (int i = t; i < nm; i += kThreads) {
-    const int to = holes[i], from = movers[i];
-    w_out[to] = w_in[from];
-    pos_out[to] = position(from);
-  }
-  for (int i = t; i < nm * chunks; i += kThreads) {
-    const int to = holes[i / chunks], from = movers[i / chunks], c = i % chunks;
-    const int pt = table[to / attn::kBS], pf = table[from / attn::kBS];
-    if (pt < 0 || pt >= p.pool_blocks || pf < 0 || pf >= p.pool_blocks) {
-      atomicOr(p.status, kStatusBadIndex);
-      continue;
+  // thread t takes words [t q, t q + q): ranks follow the slot order
+  const int q = (seg / 32 + NT - 1) / NT;
+  const int wa = min(t * q, words), wb = min(wa + q, words);
+  if (!all_equal) {
+    uint32_t c = 0, all;
+    for (int i = wa; i < wb; ++i) c += __popc(equal_w[i]);
+    int tie = int(scan_before<NT>(c, sh.warp_sum, all));
+    if (C > 1) {
+      if (t == 0) sh.counts[0] = all;
+      cluster_sync();
+      for (int r = 0; r < part; ++r) tie += int(peer_u32(&sh.counts[0], r));
     }
-    const size_t dst = ((size_t(pt) * p.num_kv_heads + h) * attn::kBS + to % attn::kBS) * p.row_bytes + 16 * c;
-    const size_t src = ((size_t(pf) * p.num_kv_heads + h) * attn::kBS + from % attn::kBS) * p.row_bytes + 16 * c;
-    *reinterpret_cast<uint4 *>(p.k_pool + dst) = *reinterpret_cast<const uint4 *>(p.k_pool + src);
-    *reinterpret_cast<uint4 *>(p.v_pool + dst) = *reinterpret_cast<const uint4 *>(p.v_pool + src);
+    for (int i = wa; i < wb; ++i) {
+      const uint32_t eq = equal_w[i];
+      stay[i] |= lowest_bits(eq, left - tie);
+      tie += __popc(eq);
+    }
+    __syncthreads();  // warp_sum is used again
   }
-  __syncthreads();  // weights of the movers are read: weight_out may be weight_in
-  for (int j = p.keep + t; j < n; j += kThreads) w_out[j] = 0.f;
+  auto below_keep = [&](int i) { return low_bits(p.keep - s0 - 32 * i); };  // slots of word i that are below keep
+  auto live = [&](int i) { return low_bits(len - 32 * i); };
+  uint32_t cnt = 0, all;
+  for (int i = wa; i < wb; ++i)
+    cnt += __popc(live(i) & below_keep(i) & ~stay[i]) + (__popc(stay[i] & ~below_keep(i)) << 16);
+  const uint32_t rank = scan_before<NT>(cnt, sh.warp_sum, all);
+  int rank_h = rank & 0xffff, rank_m = rank >> 16, moves = all >> 16;
+  if (C > 1) {
+    if (t == 0) sh.counts[1] = all;
+    cluster_sync();
+    moves = 0;
+    for (int r = 0; r < C; ++r) {
+      const uint32_t c = peer_u32(&sh.counts[1], r);
+      if (r < part) {
+        rank_h += c & 0xffff;
+        rank_m += c >> 16;
+      }
+      moves += c >> 16;
+    }
+  }
+  if (part == 0 && t == 0) p.moves[pair] = moves;
+  int32_t *holes = p.lists + pair * 2 * size_t(p.half), *movers = holes + p.half;
+  for (int i = wa; i < wb; ++i) {
+    const uint32_t s = stay[i], lo = below_keep(i);
+    equal_w[i] = rank_m;
+    hole0[i] = rank_h;
+    rank_m += __popc(s & ~lo);
+    rank_h += __popc(live(i) & lo & ~s);
+  }
+  __syncthreads();
+  // the lists, and the weights and positions of the slots that do not move
+  const bool same_w = p.w_in == p.w_out, same_pos = p.pos_in == p.pos_out;
+#pragma unroll 4
+  for (int j = s0 + t; j < s1; j += NT) {
+    const int i = (j - s0) >> 5;
+    const uint32_t s = stay[i], bit = 1u << (j & 31);  // s0 is a multiple of 32
+    if (j < p.keep) {
+      if (s & bit) {
+        if (!same_w) w_out[j] = w_in[j];
+        if (!same_pos || j >= known) pos_out[j] = position(j);
+      } else {
+        holes[hole0[i] + __popc(~s & (bit - 1))] = j;
+      }
+    } else {
+      if (s & bit) movers[equal_w[i] + __popc(s & ~below_keep(i) & (bit - 1))] = j;
+      else w_out[j] = 0.f;
+    }
+  }
+  if (C > 1) cluster_sync();  // no CTA leaves while another may read its shared memory
+}
+
+constexpr int kMoveThreads = 128;
+
+// Moves `first`.. of one (sequence, kv head): each warp looks up the pages of 4 x `per` moves, a
+// lane each, which also takes the mover's weight and position along, then copies their K and V
+// rows, every load before the first store.
+__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(EvictParams p) {
+  const int row = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 31;
+  const size_t pair = size_t(row) * p.num_kv_heads + h;
+  const int per = 32 / p.chunks, sub = lane / p.chunks, ch = lane % p.chunks;  // chunks: 8, 16 or 32
+  const int step = 4 * per;
+  const int r0 = (int(blockIdx.z) * (kMoveThreads / 32) + int(threadIdx.x >> 5)) * step;
+  const int32_t *holes = p.lists + pair * 2 * size_t(p.half), *movers = holes + p.half;
+  const bool mine = lane < step && r0 + lane < p.half;
+  const int jt = mine ? holes[r0 + lane] : 0, jf = mine ? movers[r0 + lane] : 0;  // beside the count, not behind it
+  const int count = p.moves[pair] - r0;  // (0 for a row that was skipped)
+  if (count <= 0) return;
+  const int n = p.row_ctx[row], trow = p.row_table ? p.row_table[row] : row;
+  const int known = p.row_known ? p.row_known[row] : 0;
+  long long to = -1, from = -1;  // row of the pool, -1 where there is nothing to copy
+  if (mine && lane < count) {
+    const int32_t *table = p.block_tables + size_t(trow) * p.max_blocks_per_seq;
+    const int pt = table[jt / kBS], pf = table[jf / kBS];
+    const size_t base = (size_t(trow) * p.num_kv_heads + h) * size_t(p.stride);
+    const float w = p.w_in[base + jf];
+    const int pos = jf < known ? p.pos_in[base + jf] : p.row_next[row] - n + jf;
+    if (pt >= 0 && pt < p.pool_blocks && pf >= 0 && pf < p.pool_blocks) {
+      to = ((long long)(pt) * p.num_kv_heads + h) * kBS + jt % kBS;
+      from = ((long long)(pf) * p.num_kv_heads + h) * kBS + jf % kBS;
+    } else {
+      atomicOr(p.status, kStatusBadIndex);
+    }
+    p.w_out[base + jt] = w;
+    p.w_out[base + jf] = 0.f;
+    p.pos_out[base + jt] = pos;
+  }
+  uint4 kv[4], vv[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const long long src = __shfl_sync(kFull, from, u * per + sub);
+    if (src >= 0) {
+      kv[u] = reinterpret_cast<const uint4 *>(p.k_pool)[src * p.chunks + ch];
+      vv[u] = reinterpret_cast<const uint4 *>(p.v_pool)[src * p.chunks + ch];
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const long long dst = __shfl_sync(kFull, to, u * per + sub);
+    if (dst >= 0) {
+      reinterpret_cast<uint4 *>(p.k_pool)[dst * p.chunks + ch] = kv[u];
+      reinterpret_cast<uint4 *>(p.v_pool)[dst * p.chunks + ch] = vv[u];
+    }
+  }
+}
+
+// CTAs per (sequence, kv head): enough to fill the machine (two on each of the 148 SMs), with
+// at least 4096 slots each (a cluster barrier costs as much as 4096 slots' share of a digit),
+// and as many as the rank keys need.
+int evict_cluster(int rows, int hkv, int max_ctx) {
+  int c = 1;
+  while (c < kMaxCluster &&
+         (max_ctx > c * kMaxSlots || ((long long)rows * hkv * c < 2 * 148 && max_ctx > 4096 * c)))
+    c *= 2;
+  return c;
+}
+
+size_t evict_smem(int seg) { return (size_t(seg) + 3 * (seg / 32)) * sizeof(uint32_t); }
+
+template <int NT>
+cudaError_t launch_evict(const EvictParams &p, int rows, int C, cudaStream_t stream) {
+  auto kern = evict_kernel<NT>;
+  const int seg = ((p.max_ctx + C - 1) / C + 31) / 32 * 32;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(evict_smem(kMaxSlots)));
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(rows) * C, p.num_kv_heads);
+  cfg.blockDim = dim3(NT);
+  cfg.dynamicSmemBytes = evict_smem(seg);
+  cfg.stream = stream;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = C;
+  at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = C > 1 ? 1 : 0;
+  e = cudaLaunchKernelEx(&cfg, kern, p, C, seg);
+  if (e != cudaSuccess) return e;
+  const int most = std::min(p.keep, p.max_ctx - p.keep);  // moves of one head
+  if (most <= 0) return cudaSuccess;
+  const int per_cta = kMoveThreads / 32 * 4 * (32 / p.chunks);
+  const dim3 grid(rows, p.num_kv_heads, (most + per_cta - 1) / per_cta);
+  evict_move_kernel<<<grid, kMoveThreads, 0, stream>>>(p);
+  return cudaGetLastError();
 }
 
 }  // namespace
 
 int64_t evict_workspace_bytes(int num_rows, int num_kv_heads, int max_ctx) {
   if (num_rows <= 0 || num_kv_heads <= 0 || max_ctx <= 0) return 0;
-  return int64_t(num_rows) * num_kv_heads * 2 * max_ctx * int64_t(sizeof(int32_t));
+  // holes and movers (at most half of the slots each) and their number
+  return int64_t(num_rows) * num_kv_heads * (2 * (max_ctx / 2 + 1) + 1) * int64_t(sizeof(int32_t));
 }
 
 }  // namespace ms
@@ -180,7 +450,7 @@ extern "C" int ms_launch_evict(void *k_pool, void *v_pool, int64_t pool_blocks, 
   if (num_rows == 0 || max_ctx == 0) return 0;
   if (!head_layout_ok(num_kv_heads, num_kv_heads, head_dim, block_size, dtype) || num_kv_heads > 65535 ||
       !pools_ok(k_pool, v_pool, pool_blocks, num_kv_heads, block_tables, table_rows, max_blocks_per_seq) ||
-      max_ctx > kMaxSlots || max_ctx > int64_t(max_blocks_per_seq) * attn::kBS || stride < max_ctx ||
+      max_ctx > kMaxCluster * kMaxSlots || max_ctx > int64_t(max_blocks_per_seq) * attn::kBS || stride < max_ctx ||
       (!row_table && table_rows < num_rows) || !row_ctx || !row_next || (row_known && !pos_in) || !weight_in ||
       !weight_out || !pos_out || keep <= 0 || sinks < 0 || recent < 0 || int64_t(sinks) + recent > keep ||
       workspace == nullptr || workspace_bytes < evict_workspace_bytes(num_rows, num_kv_heads, max_ctx))
@@ -196,7 +466,6 @@ extern "C" int ms_launch_evict(void *k_pool, void *v_pool, int64_t pool_blocks, 
   p.row_ctx = row_ctx;
   p.row_next = row_next;
   p.row_known = row_known;
-  p.num_rows = num_rows;
   p.max_ctx = max_ctx;
   p.keep = keep;
   p.sinks = sinks;
@@ -207,13 +476,16 @@ extern "C" int ms_launch_evict(void *k_pool, void *v_pool, int64_t pool_blocks, 
   p.pos_out = pos_out;
   p.stride = stride;
   p.num_kv_heads = num_kv_heads;
-  p.row_bytes = head_dim * (dtype == MS_DTYPE_F32 ? 4 : 2);
+  p.chunks = head_dim * (dtype == MS_DTYPE_F32 ? 4 : 2) / 16;
+  p.half = max_ctx / 2 + 1;
   p.lists = static_cast<int32_t *>(workspace);
+  p.moves = p.lists + size_t(num_rows) * num_kv_heads * 2 * p.half;
   cudaError_t e = standalone_status_word(&p.status);
   if (e != cudaSuccess) return int(e);
-  const size_t smem = size_t(max_ctx) * sizeof(uint32_t);
-  e = cudaFuncSetAttribute(evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSlots * 4);
-  if (e != cudaSuccess) return int(e);
-  evict_kernel<<<dim3(num_rows, num_kv_heads), kThreads, smem, static_cast<cudaStream_t>(stream)>>>(p);
-  return int(cudaGetLastError());
+  const int C = evict_cluster(num_rows, num_kv_heads, max_ctx);
+  if ((long long)num_rows * C > 0x7fffffffLL) return int(cudaErrorInvalidValue);
+  // small CTAs, four to an SM, where there are enough of them to fill it that way
+  const bool many = (long long)num_rows * num_kv_heads * C >= 2 * 148;
+  return int(many ? launch_evict<256>(p, num_rows, C, static_cast<cudaStream_t>(stream))
+                  : launch_evict<512>(p, num_rows, C, static_cast<cudaStream_t>(stream)));
 }

@@ -226,10 +226,6 @@ __device__ __forceinline__ void exp2_poly2(float &y0, float &y1, float x0, float
   y0 = __int_as_float(__float_as_int(p0) + (__float_as_int(t0) << 23));
   y1 = __int_as_float(__float_as_int(p1) + (__float_as_int(t1) << 23));
 }
-// bits 0 .. n - 1 set (none for n <= 0, all from n = 32 on)
-__device__ __forceinline__ uint32_t keys_below(int n) {
-  return n <= 0 ? 0u : 0xffffffffu >> (32 - min(n, 32));
-}
 __device__ __forceinline__ float ex2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -426,7 +422,7 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
       auto visible_bits = [&](auto masked, int k) -> uint32_t {
         if constexpr (WIN && decltype(masked)::value) {
           const int base = key0 + 32 * k;
-          return keys_below(pos + 1 - base) & (~keys_below(lo - base) | keys_below(p.sinks - base));
+          return low_bits(pos + 1 - base) & (~low_bits(lo - base) | low_bits(p.sinks - base));
         }
         return 0u;
       };

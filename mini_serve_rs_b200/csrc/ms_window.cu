@@ -54,9 +54,6 @@ struct RowsParams {
   int wait_limit;
 };
 
-// bits 0 .. n - 1 set (none for n <= 0, all from n = 32 on)
-__device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : 0xffffffffu >> (32 - min(n, 32)); }
-
 // ---- one page of one kv head: 16-bit K/V on mma.sync ----------------------------------
 template <typename T_, int D_, int NSTAGE_> struct PageTc {
   using T = T_;
@@ -302,24 +299,6 @@ template <int D_, int G> struct PageF32 {
   }
 };
 
-// ---- clusters ------------------------------------------------------------------------------
-__device__ __forceinline__ void cluster_arrive() {
-  __syncwarp();
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void cluster_wait() {
-  __syncwarp();
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// the f32 / i32 at `p` (this CTA's shared memory) in CTA `rank` of the cluster
-__device__ __forceinline__ float peer_f32(const float *p, int rank) {
-  uint32_t a;
-  float v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(p)), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
-  return v;
-}
-
 constexpr int kMaxGroup = 8;
 
 // Page::D * kMaxGroup floats for each warp's O and the CTA's; the maxima and sums of both
@@ -404,7 +383,7 @@ __global__ void __launch_bounds__(kWarps * 32)
     }
     const int key0 = vis.page_at(b0 + warp + k * kWarps) * kBS;
     const uint32_t bits =
-        0xffffu & bits_below(ctx - key0) & (~bits_below(low - key0) | bits_below(p.sinks - key0));
+        0xffffu & low_bits(ctx - key0) & (~low_bits(low - key0) | low_bits(p.sinks - key0));
     pg.page(my_stage + size_t(s) * STAGE_BYTES, bits, p.qscale, WEIGHTS ? raw + key0 : nullptr, p.ctx16, G);
     __syncwarp();
     if (issued < nb_w && k + NSTAGE == issued) {

@@ -42,6 +42,43 @@ __device__ __forceinline__ bool table_row_repeated(const int32_t *row_table, int
   return __syncthreads_or(found) != 0;
 }
 
+// bits 0 .. n - 1 set (none for n <= 0, all from n = 32 on)
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : 0xffffffffu >> (32 - min(n, 32)); }
+
+// ---- thread-block clusters ------------------------------------------------------
+__device__ __forceinline__ void cluster_arrive() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+  cluster_arrive();
+  cluster_wait();
+}
+// the 32-bit value at `p` (this CTA's shared memory) in CTA `rank` of the cluster
+__device__ __forceinline__ uint32_t peer_u32(const uint32_t *p, int rank) {
+  uint32_t a, v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(attn::smem_addr(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint4 peer_u4(const uint32_t *p, int rank) {
+  uint32_t a;
+  uint4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(attn::smem_addr(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(a)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ float peer_f32(const float *p, int rank) {
+  return __uint_as_float(peer_u32(reinterpret_cast<const uint32_t *>(p), rank));
+}
+
 inline bool head_layout_ok(int num_heads, int num_kv_heads, int head_dim, int block_size, int dtype) {
   if (num_kv_heads <= 0 || num_heads <= 0 || num_heads % num_kv_heads != 0 || block_size != attn::kBS) return false;
   const int g = num_heads / num_kv_heads;

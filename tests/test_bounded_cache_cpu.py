@@ -71,7 +71,7 @@ def test_attention_weights_refuses(bad):
 
 @pytest.mark.parametrize("bad", COMMON + [
     dict(ctx=None), dict(next=None), dict(pos=None), dict(w=None), dict(w_out=None), dict(pos_out=None), dict(stride=599),
-    dict(max_ctx=641), dict(max_ctx=-1), dict(blocks=1 << 20, max_ctx=49153, stride=49153), dict(keep=0), dict(keep=-1),
+    dict(max_ctx=641), dict(max_ctx=-1), dict(blocks=1 << 20, max_ctx=262145, stride=262145), dict(keep=0), dict(keep=-1),
     dict(recent=-1), dict(sinks=401), dict(recent=497), dict(sinks=2 ** 31 - 1, recent=2 ** 31 - 1), dict(ws=None),
     dict(ws_bytes=0), dict(row_table=None, n=9)], ids=str)
 def test_evict_refuses(bad):
@@ -90,4 +90,4 @@ def test_workspace_formulas():
     for r, h, c in ((1, 16, 1), (64, 28, 4097), (256, 32, 131072)):
         assert lib.ms_attention_weights_workspace_bytes(r, h, c) >= 4 * r * h * c
     assert lib.ms_evict_workspace_bytes(0, 8, 100) == 0
-    assert lib.ms_evict_workspace_bytes(256, 8, 49152) > 0
+    assert lib.ms_evict_workspace_bytes(256, 8, 262144) > 0

@@ -146,7 +146,8 @@ def test_ties_and_special_weights(kind):
     run(s, 500, 3, 40, s["ctx"], None, torch.bfloat16, True)
 
 
-@pytest.mark.parametrize("ctx,keep", [([5000, 4097], 4096), ([20000], 513), ([9000, 33], 8999)])
+@pytest.mark.parametrize("ctx,keep", [([5000, 4097], 4096), ([20000], 513), ([9000, 33], 8999), ([70000, 40000], 30001),
+                                      ([140001], 1000), ([262144], 130000)])
 def test_long(ctx, keep):
     s = state(ctx, 2, 64, torch.float16, keep)
     run(s, keep, 4, min(200, keep // 2), ctx, None, torch.float16, True)
