@@ -161,7 +161,53 @@ __device__ __forceinline__ uint32_t lowest_bits(uint32_t w, int n) {
   return out;
 }
 
-template <int NT>
+// Moves [r0, r0 + moves_per_warp()) of one head, as far as there are `count`, by one warp: a lane
+// each looks up the pages and takes the mover's weight and position along, then their K and V
+// rows are copied, every load before the first store.  jt, jf: the lane's hole and mover.
+__device__ __forceinline__ int moves_per_warp(const EvictParams &p) { return 4 * (32 / p.chunks); }
+__device__ __forceinline__ void move_rows(const EvictParams &p, int row, int h, int jt, int jf, int count) {
+  const int lane = threadIdx.x & 31;
+  const int per = 32 / p.chunks, sub = lane / p.chunks, ch = lane % p.chunks;  // chunks: 8, 16 or 32
+  long long to = -1, from = -1;  // row of the pool, -1 where there is nothing to copy
+  if (lane < min(count, 4 * per)) {
+    const int n = p.row_ctx[row], trow = p.row_table ? p.row_table[row] : row;
+    const int known = p.row_known ? p.row_known[row] : 0;
+    const int32_t *table = p.block_tables + size_t(trow) * p.max_blocks_per_seq;
+    const int pt = table[jt / kBS], pf = table[jf / kBS];
+    const size_t base = (size_t(trow) * p.num_kv_heads + h) * size_t(p.stride);
+    const float w = p.w_in[base + jf];
+    const int pos = jf < known ? p.pos_in[base + jf] : p.row_next[row] - n + jf;
+    if (pt >= 0 && pt < p.pool_blocks && pf >= 0 && pf < p.pool_blocks) {
+      to = ((long long)(pt) * p.num_kv_heads + h) * kBS + jt % kBS;
+      from = ((long long)(pf) * p.num_kv_heads + h) * kBS + jf % kBS;
+    } else {
+      atomicOr(p.status, kStatusBadIndex);
+    }
+    p.w_out[base + jt] = w;
+    p.w_out[base + jf] = 0.f;  // after it was read: weight_out may be weight_in
+    p.pos_out[base + jt] = pos;
+  }
+  uint4 kv[4], vv[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const long long src = __shfl_sync(kFull, from, u * per + sub);
+    if (src >= 0) {
+      kv[u] = reinterpret_cast<const uint4 *>(p.k_pool)[src * p.chunks + ch];
+      vv[u] = reinterpret_cast<const uint4 *>(p.v_pool)[src * p.chunks + ch];
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const long long dst = __shfl_sync(kFull, to, u * per + sub);
+    if (dst >= 0) {
+      reinterpret_cast<uint4 *>(p.k_pool)[dst * p.chunks + ch] = kv[u];
+      reinterpret_cast<uint4 *>(p.v_pool)[dst * p.chunks + ch] = vv[u];
+    }
+  }
+}
+
+// FUSED: the cluster's warps also make the moves.
+template <int NT, bool FUSED>
 __global__ void __launch_bounds__(NT, 1024 / NT) evict_kernel(EvictParams p, int C, int seg) {
   constexpr int kWarpsNT = NT / 32;
   // [seg] rank keys, then [seg / 32] words three times
@@ -311,20 +357,42 @@ __global__ void __launch_bounds__(NT, 1024 / NT) evict_kernel(EvictParams p, int
   __syncthreads();
   // the lists, and the weights and positions of the slots that do not move
   const bool same_w = p.w_in == p.w_out, same_pos = p.pos_in == p.pos_out;
-#pragma unroll 4
-  for (int j = s0 + t; j < s1; j += NT) {
-    const int i = (j - s0) >> 5;
-    const uint32_t s = stay[i], bit = 1u << (j & 31);  // s0 is a multiple of 32
-    if (j < p.keep) {
-      if (s & bit) {
-        if (!same_w) w_out[j] = w_in[j];
-        if (!same_pos || j >= known) pos_out[j] = position(j);
+  constexpr int V = 6;  // weights of V slots per thread under way at once
+  for (int j0 = s0 + t; j0 < s1; j0 += V * NT) {
+    float w[V];
+    int pos[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int j = j0 + v * NT;
+      const bool in_place = j < min(p.keep, s1) && (stay[(j - s0) >> 5] >> (j & 31) & 1);  // s0 is a multiple of 32
+      w[v] = in_place && !same_w ? w_in[j] : 0.f;
+      pos[v] = in_place && !(same_pos && j < known) ? position(j) : 0;
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int j = j0 + v * NT, i = (j - s0) >> 5;
+      if (j >= s1) break;
+      const uint32_t s = stay[i], bit = 1u << (j & 31);
+      if (j < p.keep) {
+        if (s & bit) {
+          if (!same_w) w_out[j] = w[v];
+          if (!(same_pos && j < known)) pos_out[j] = pos[v];
+        } else {
+          holes[hole0[i] + __popc(~s & (bit - 1))] = j;
+        }
       } else {
-        holes[hole0[i] + __popc(~s & (bit - 1))] = j;
+        if (s & bit) movers[equal_w[i] + __popc(s & ~below_keep(i) & (bit - 1))] = j;
+        else w_out[j] = 0.f;
       }
-    } else {
-      if (s & bit) movers[equal_w[i] + __popc(s & ~below_keep(i) & (bit - 1))] = j;
-      else w_out[j] = 0.f;
+    }
+  }
+  if constexpr (FUSED) {
+    if (C > 1) cluster_sync();
+    else __syncthreads();
+    const int step = moves_per_warp(p);
+    for (int r0 = (part * kWarpsNT + warp) * step; r0 < moves; r0 += C * kWarpsNT * step) {
+      const bool mine = r0 + lane < moves;
+      move_rows(p, row, h, mine ? holes[r0 + lane] : 0, mine ? movers[r0 + lane] : 0, moves - r0);
     }
   }
   if (C > 1) cluster_sync();  // no CTA leaves while another may read its shared memory
@@ -332,56 +400,15 @@ __global__ void __launch_bounds__(NT, 1024 / NT) evict_kernel(EvictParams p, int
 
 constexpr int kMoveThreads = 128;
 
-// Moves `first`.. of one (sequence, kv head): each warp looks up the pages of 4 x `per` moves, a
-// lane each, which also takes the mover's weight and position along, then copies their K and V
-// rows, every load before the first store.
 __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(EvictParams p) {
-  const int row = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 31;
+  const int row = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 31, step = moves_per_warp(p);
   const size_t pair = size_t(row) * p.num_kv_heads + h;
-  const int per = 32 / p.chunks, sub = lane / p.chunks, ch = lane % p.chunks;  // chunks: 8, 16 or 32
-  const int step = 4 * per;
   const int r0 = (int(blockIdx.z) * (kMoveThreads / 32) + int(threadIdx.x >> 5)) * step;
   const int32_t *holes = p.lists + pair * 2 * size_t(p.half), *movers = holes + p.half;
   const bool mine = lane < step && r0 + lane < p.half;
   const int jt = mine ? holes[r0 + lane] : 0, jf = mine ? movers[r0 + lane] : 0;  // beside the count, not behind it
-  const int count = p.moves[pair] - r0;  // (0 for a row that was skipped)
-  if (count <= 0) return;
-  const int n = p.row_ctx[row], trow = p.row_table ? p.row_table[row] : row;
-  const int known = p.row_known ? p.row_known[row] : 0;
-  long long to = -1, from = -1;  // row of the pool, -1 where there is nothing to copy
-  if (mine && lane < count) {
-    const int32_t *table = p.block_tables + size_t(trow) * p.max_blocks_per_seq;
-    const int pt = table[jt / kBS], pf = table[jf / kBS];
-    const size_t base = (size_t(trow) * p.num_kv_heads + h) * size_t(p.stride);
-    const float w = p.w_in[base + jf];
-    const int pos = jf < known ? p.pos_in[base + jf] : p.row_next[row] - n + jf;
-    if (pt >= 0 && pt < p.pool_blocks && pf >= 0 && pf < p.pool_blocks) {
-      to = ((long long)(pt) * p.num_kv_heads + h) * kBS + jt % kBS;
-      from = ((long long)(pf) * p.num_kv_heads + h) * kBS + jf % kBS;
-    } else {
-      atomicOr(p.status, kStatusBadIndex);
-    }
-    p.w_out[base + jt] = w;
-    p.w_out[base + jf] = 0.f;
-    p.pos_out[base + jt] = pos;
-  }
-  uint4 kv[4], vv[4];
-#pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const long long src = __shfl_sync(kFull, from, u * per + sub);
-    if (src >= 0) {
-      kv[u] = reinterpret_cast<const uint4 *>(p.k_pool)[src * p.chunks + ch];
-      vv[u] = reinterpret_cast<const uint4 *>(p.v_pool)[src * p.chunks + ch];
-    }
-  }
-#pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const long long dst = __shfl_sync(kFull, to, u * per + sub);
-    if (dst >= 0) {
-      reinterpret_cast<uint4 *>(p.k_pool)[dst * p.chunks + ch] = kv[u];
-      reinterpret_cast<uint4 *>(p.v_pool)[dst * p.chunks + ch] = vv[u];
-    }
-  }
+  const int count = p.moves[pair] - r0;  // (0 moves for a row that was skipped)
+  if (count > 0) move_rows(p, row, h, jt, jf, count);
 }
 
 // CTAs per (sequence, kv head): enough to fill the machine (two on each of the 148 SMs), with
@@ -397,12 +424,19 @@ int evict_cluster(int rows, int hkv, int max_ctx) {
 
 size_t evict_smem(int seg) { return (size_t(seg) + 3 * (seg / 32)) * sizeof(uint32_t); }
 
-template <int NT>
+template <int NT, bool FUSED>
 cudaError_t launch_evict(const EvictParams &p, int rows, int C, cudaStream_t stream) {
-  auto kern = evict_kernel<NT>;
+  auto kern = evict_kernel<NT, FUSED>;
   const int seg = ((p.max_ctx + C - 1) / C + 31) / 32 * 32;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(evict_smem(kMaxSlots)));
-  if (e != cudaSuccess) return e;
+  static std::atomic<bool> attr_done[64];  // per device; zero-initialised (static storage)
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !attr_done[dev].load(std::memory_order_acquire)) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(evict_smem(kMaxSlots)));
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64) attr_done[dev].store(true, std::memory_order_release);  // setting twice is harmless
+  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(rows) * C, p.num_kv_heads);
   cfg.blockDim = dim3(NT);
@@ -414,10 +448,10 @@ cudaError_t launch_evict(const EvictParams &p, int rows, int C, cudaStream_t str
   at.val.clusterDim.y = at.val.clusterDim.z = 1;
   cfg.attrs = &at;
   cfg.numAttrs = C > 1 ? 1 : 0;
-  e = cudaLaunchKernelEx(&cfg, kern, p, C, seg);
-  if (e != cudaSuccess) return e;
-  const int most = std::min(p.keep, p.max_ctx - p.keep);  // moves of one head
-  if (most <= 0) return cudaSuccess;
+  return cudaLaunchKernelEx(&cfg, kern, p, C, seg);
+}
+
+cudaError_t launch_moves(const EvictParams &p, int rows, int most, cudaStream_t stream) {
   const int per_cta = kMoveThreads / 32 * 4 * (32 / p.chunks);
   const dim3 grid(rows, p.num_kv_heads, (most + per_cta - 1) / per_cta);
   evict_move_kernel<<<grid, kMoveThreads, 0, stream>>>(p);
@@ -484,8 +518,14 @@ extern "C" int ms_launch_evict(void *k_pool, void *v_pool, int64_t pool_blocks, 
   if (e != cudaSuccess) return int(e);
   const int C = evict_cluster(num_rows, num_kv_heads, max_ctx);
   if ((long long)num_rows * C > 0x7fffffffLL) return int(cudaErrorInvalidValue);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int most = std::max(0, std::min(keep, max_ctx - keep));  // moves of one head
+  // One launch where every warp of the cluster has at most one round of moves: a second launch
+  // costs the host 5 us and the GPU 1 us.
+  if ((long long)most <= C * (512LL / 32) * 4 * (32 / p.chunks)) return int(launch_evict<512, true>(p, num_rows, C, st));
   // small CTAs, four to an SM, where there are enough of them to fill it that way
   const bool many = (long long)num_rows * num_kv_heads * C >= 2 * 148;
-  return int(many ? launch_evict<256>(p, num_rows, C, static_cast<cudaStream_t>(stream))
-                  : launch_evict<512>(p, num_rows, C, static_cast<cudaStream_t>(stream)));
+  e = many ? launch_evict<256, false>(p, num_rows, C, st) : launch_evict<512, false>(p, num_rows, C, st);
+  if (e == cudaSuccess) e = launch_moves(p, num_rows, most, st);
+  return int(e);
 }
