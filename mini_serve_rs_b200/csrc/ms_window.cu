@@ -12,8 +12,11 @@
 // kv head); CTA c takes the c-th share of the row's visible pages (sink pages,
 // then the window's; the others are never touched), its 4 warps take the
 // share's pages in turn, each through a private ring of shared-memory stages
-// filled by TMA (no multicast) on per-stage mbarriers.  One read of K and V
-// serves all query heads of the kv head:
+// filled by TMA (no multicast) on per-stage mbarriers.  Two stages a warp and
+// three CTAs on an SM: 192 KB of copies in flight, and while one CTA joins its
+// warps the others stream (three stages and two CTAs: 86 against 79 us on 64
+// rows of 28/4 heads behind a 4096-token window, 0.97 of the copy rate).
+// One read of K and V serves all query heads of the kv head:
 //  * 16-bit: the heads are rows 0..G-1 of an m16 tile, S = Q K^T and O += P V
 //    as mma.sync.m16n8k16 on the swizzled tile (16 x 16 x D per page is far
 //    below one tcgen05 tile), online softmax in base 2 on the four scores a
@@ -37,7 +40,7 @@ namespace {
 
 using namespace attn;
 
-constexpr int kMaxCluster = 16;
+constexpr int kMaxCluster = 8;
 
 struct RowsParams {
   const void *q, *k_pool, *v_pool;
@@ -55,9 +58,9 @@ struct RowsParams {
 };
 
 // ---- one page of one kv head: 16-bit K/V on mma.sync ----------------------------------
-template <typename T_, int D_, int NSTAGE_> struct PageTc {
+template <typename T_, int D_> struct PageTc {
   using T = T_;
-  static constexpr int D = D_, NSTAGE = NSTAGE_;
+  static constexpr int D = D_, WARPS = 4, NSTAGE = D == 128 ? 2 : 3;
   static constexpr int NDH = D / 64, TILE_BYTES = NDH * kHalfBytes, KSTEPS = D / 16, NTD = D / 8;
   uint32_t qa[KSTEPS][2];
   float o[NTD][4];
@@ -98,17 +101,23 @@ template <typename T_, int D_, int NSTAGE_> struct PageTc {
         if (!(bits >> ((i >> 3) & 15) & 1)) vz[i] = make_uint4(0u, 0u, 0u, 0u);
       __syncwarp();
     }
+    // tokens 0..7 and 8..15; even and odd k-steps apart: half the chain of dependent products
     float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    float sd[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-    for (int kk = 0; kk < KSTEPS; ++kk) {
-      uint32_t b[4];
+    for (int kk = 0; kk < KSTEPS; kk += 2) {
+      uint32_t b[4], c[4];
       ldmatrix_x4(b, kb + tile_off((mi >> 1) * 8 + lr, kk * 16 + (mi & 1) * 8));
+      ldmatrix_x4(c, kb + tile_off((mi >> 1) * 8 + lr, kk * 16 + 16 + (mi & 1) * 8));
       const uint32_t a[4] = {qa[kk][0], 0u, qa[kk][1], 0u};
+      const uint32_t a2[4] = {qa[kk + 1][0], 0u, qa[kk + 1][1], 0u};
       mma_16816<T>(sc[0], a, b[0], b[1]);
       mma_16816<T>(sc[1], a, b[2], b[3]);
+      mma_16816<T>(sd[0], a2, c[0], c[1]);
+      mma_16816<T>(sd[1], a2, c[2], c[3]);
     }
     // row gid: tokens 2 tig, 2 tig + 1, 8 + 2 tig, 9 + 2 tig
-    float sv[4] = {sc[0][0], sc[0][1], sc[1][0], sc[1][1]};
+    float sv[4] = {sc[0][0] + sd[0][0], sc[0][1] + sd[0][1], sc[1][0] + sd[1][0], sc[1][1] + sd[1][1]};
     float mx = -INFINITY;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -169,7 +178,7 @@ template <typename T_, int D_, int NSTAGE_> struct PageTc {
 // ---- one page of one kv head: f32 on the FMA pipe ---------------------------------------
 template <int D_, int G> struct PageF32 {
   using T = float;
-  static constexpr int D = D_, NSTAGE = D == 128 ? 2 : 3;
+  static constexpr int D = D_, WARPS = 2, NSTAGE = D == 128 ? 2 : 3;
   static constexpr int DPL = D / 32, TILE = kBS * D, TILE_BYTES = TILE * 4;
   static constexpr int SUB = (G > 4) ? 8 : 16;  // tokens per scoring sub-tile
   static constexpr int NV = G * SUB, NVP = ((NV + 31) / 32) * 32;
@@ -303,17 +312,18 @@ constexpr int kMaxGroup = 8;
 
 // Page::D * kMaxGroup floats for each warp's O and the CTA's; the maxima and sums of both
 template <class Page> struct Layout {
-  static constexpr size_t kStages = size_t(kWarps) * Page::NSTAGE * 2 * Page::TILE_BYTES;
-  static constexpr size_t kBars = kWarps * Page::NSTAGE * sizeof(uint64_t);
-  static constexpr size_t kMerge = (size_t(kWarps) + 1) * kMaxGroup * (Page::D + 2) * sizeof(float);
+  static constexpr int W = Page::WARPS;
+  static constexpr size_t kStages = size_t(W) * Page::NSTAGE * 2 * Page::TILE_BYTES;
+  static constexpr size_t kBars = W * Page::NSTAGE * sizeof(uint64_t);
+  static constexpr size_t kMerge = (size_t(W) + 1) * kMaxGroup * (Page::D + 2) * sizeof(float);
   static constexpr size_t kSmem = 1024 + std::max(kStages + kBars, kMerge);
 };
 
 template <class Page, bool WEIGHTS>
-__global__ void __launch_bounds__(kWarps * 32)
+__global__ void __launch_bounds__(Page::WARPS * 32)
     window_rows_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                        RowsParams p, int C) {
-  constexpr int NSTAGE = Page::NSTAGE, STAGE_BYTES = 2 * Page::TILE_BYTES, D = Page::D;
+  constexpr int W = Page::WARPS, NSTAGE = Page::NSTAGE, STAGE_BYTES = 2 * Page::TILE_BYTES, D = Page::D;
   using T = typename Page::T;
   extern __shared__ unsigned char smem_dyn[];
   unsigned char *smem =
@@ -335,7 +345,7 @@ __global__ void __launch_bounds__(kWarps * 32)
   const VisiblePages vis(ctx - 1, ctx, p.window, p.sinks);
   const int share = (vis.count + C - 1) / C;
   const int b0 = min(part * share, vis.count), b1 = min(b0 + share, vis.count);
-  const int nb_w = (b1 - b0 - warp + kWarps - 1) / kWarps;  // pages b0 + warp + k * kWarps
+  const int nb_w = (b1 - b0 - warp + W - 1) / W;  // pages b0 + warp + k * W
   unsigned char *my_stage = smem + size_t(warp) * NSTAGE * STAGE_BYTES;
   uint64_t *my_bar = bars + warp * NSTAGE;
   if (lane == 0) {
@@ -351,7 +361,7 @@ __global__ void __launch_bounds__(kWarps * 32)
     const int k = k0 + lane;
     page_reg = 0;
     if (k < nb_w) {
-      const int page = table[vis.page_at(b0 + warp + k * kWarps)];
+      const int page = table[vis.page_at(b0 + warp + k * W)];
       if (page >= 0 && page < p.pool_blocks) page_reg = page;
       else atomicOr(p.status, kStatusBadIndex);
     }
@@ -381,7 +391,7 @@ __global__ void __launch_bounds__(kWarps * 32)
       kfail = k;
       break;
     }
-    const int key0 = vis.page_at(b0 + warp + k * kWarps) * kBS;
+    const int key0 = vis.page_at(b0 + warp + k * W) * kBS;
     const uint32_t bits =
         0xffffu & low_bits(ctx - key0) & (~low_bits(low - key0) | low_bits(p.sinks - key0));
     pg.page(my_stage + size_t(s) * STAGE_BYTES, bits, p.qscale, WEIGHTS ? raw + key0 : nullptr, p.ctx16, G);
@@ -401,22 +411,22 @@ __global__ void __launch_bounds__(kWarps * 32)
   }
 
   // ---- merge the warps (the stages are free), then the cluster's CTAs ----
-  float *wo = reinterpret_cast<float *>(smem);         // [kWarps][G][D]
-  float *wm = wo + kWarps * kMaxGroup * D;             // [kWarps][kMaxGroup] maxima, then sums
-  float *wl = wm + kWarps * kMaxGroup;
-  float *co = wl + kWarps * kMaxGroup;                 // the CTA's [G][D], maxima, sums
+  float *wo = reinterpret_cast<float *>(smem);         // [W][G][D]
+  float *wm = wo + W * kMaxGroup * D;             // [W][kMaxGroup] maxima, then sums
+  float *wl = wm + W * kMaxGroup;
+  float *co = wl + W * kMaxGroup;                 // the CTA's [G][D], maxima, sums
   float *cm = co + kMaxGroup * D, *cl = cm + kMaxGroup;
   const bool any_failed = __syncthreads_or(failed ? 1 : 0) != 0;
   pg.store(wo + warp * kMaxGroup * D, wm + warp * kMaxGroup, wl + warp * kMaxGroup, G);
   __syncthreads();
   T *out = static_cast<T *>(p.out) + head0 * D;
-  for (int i = t; i < G * D; i += kWarps * 32) {
+  for (int i = t; i < G * D; i += W * 32) {
     const int h = i / D;
     float M = -INFINITY, L = 0.f, O = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) M = fmaxf(M, wm[w * kMaxGroup + h]);
+    for (int w = 0; w < W; ++w) M = fmaxf(M, wm[w * kMaxGroup + h]);
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < W; ++w) {
       const float mw = wm[w * kMaxGroup + h], f = mw == -INFINITY ? 0.f : exp2f(mw - M);
       L += f * wl[w * kMaxGroup + h];
       O += f * wo[w * kMaxGroup * D + i];
@@ -431,7 +441,7 @@ __global__ void __launch_bounds__(kWarps * 32)
   if (C > 1) {
     cluster_arrive();
     cluster_wait();
-    for (int i = part * kWarps * 32 + t; i < G * D; i += C * kWarps * 32) {
+    for (int i = part * W * 32 + t; i < G * D; i += C * W * 32) {
       const int h = i / D;
       float M = -INFINITY, L = 0.f, O = 0.f;
       bool bad = false;
@@ -468,29 +478,63 @@ __global__ void __launch_bounds__(kWarps * 32)
     __syncthreads();
     if (C > 1) cluster_arrive();
     float *sum = p.weight_sum + (size_t(trow) * p.num_kv_heads + kvh) * p.weight_stride;
-    if (wm[0] == wm[0])
-      for (int key = b0 * kBS + t; key < min(b1 * kBS, ctx); key += kWarps * 32) {
-        float add = 0.f;
-        for (int h = 0; h < G; ++h) add += exp2f(raw[size_t(h) * p.ctx16 + key] - wm[h]) * wl[h];
-        sum[key] += add;
+    // 4 keys a thread, all heads' scores and the sums under way together: the CTA streams nothing
+    // meanwhile (a key at a time this phase took a fifth of the kernel)
+    const int end = wm[0] == wm[0] ? min(b1 * kBS, ctx) : 0;
+    const bool vec = (reinterpret_cast<uintptr_t>(sum) & 15) == 0;
+    for (int key = b0 * kBS + 4 * t; key < end; key += 4 * W * 32) {
+      float4 r[kMaxGroup];
+#pragma unroll
+      for (int h = 0; h < kMaxGroup; ++h)
+        if (h < G) r[h] = *reinterpret_cast<const float4 *>(raw + size_t(h) * p.ctx16 + key);
+      const bool whole = vec && key + 4 <= end;
+      float s[4];
+      if (whole) {
+        Vec4<float>::load(sum + key, s);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i] = key + i < end ? sum[key + i] : 0.f;
       }
+      float add[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int h = 0; h < kMaxGroup; ++h)
+        if (h < G) {
+          const float m = wm[h], f = wl[h];
+          add[0] += exp2f(r[h].x - m) * f;
+          add[1] += exp2f(r[h].y - m) * f;
+          add[2] += exp2f(r[h].z - m) * f;
+          add[3] += exp2f(r[h].w - m) * f;
+        }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[i] += add[i];
+      if (whole) {
+        Vec4<float>::store(sum + key, s);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (key + i < end) sum[key + i] = s[i];
+      }
+    }
   } else {
     if (C > 1) cluster_arrive();
   }
   if (C > 1) cluster_wait();  // no CTA leaves while another may read its shared memory
 }
 
-// CTAs per (row, kv head).  A CTA keeps 96 KB of copies in flight and two fit an SM, so the
-// machine is full from 2 x 148 CTAs on; fewer (row, kv head) pairs than that are split, down to
-// two pages a warp and to the 16 CTAs that a cluster holds.
-int cluster_size(int rows, int hkv, int max_pages) {
-  int c = 1;
-  while (c < kMaxCluster && (long long)rows * hkv * c < 2 * 148 && max_pages > 2 * kWarps * c) c *= 2;
-  return c;
+// CTAs per (row, kv head); `slots`: CTAs that the machine holds at once.  Fewer pairs than slots
+// are split to fill one wave (12 rows x 4 heads of 16k keys with weights: 8 CTAs each 70 us, 1 each
+// 243 us), down to two pages a warp and to a cluster of 8 (16, the most there is, measured slower
+// for one row: 7.1 against 6.6 us).  Between one and four waves of whole rows, halves even out
+// ragged lengths (64 rows x 8 heads: 154 against 169 us); more rows do that by themselves.
+int cluster_size(int rows, int hkv, int max_pages, int warps, int slots) {
+  const long long pairs = (long long)rows * hkv;
+  long long c = pairs > slots ? (pairs < 4 * slots ? 2 : 1) : slots / pairs;
+  c = std::min<long long>(c, kMaxCluster);
+  return int(std::max<long long>(1, std::min<long long>(c, max_pages / (2 * warps))));
 }
 
 template <class Page, bool WEIGHTS>
-cudaError_t launch_rows(const RowsParams &p, int rows, int C, const CUtensorMap &km, const CUtensorMap &vm,
+cudaError_t launch_rows(const RowsParams &p, int rows, int max_pages, const CUtensorMap &km, const CUtensorMap &vm,
                         cudaStream_t stream) {
   auto kern = window_rows_kernel<Page, WEIGHTS>;
   static std::atomic<bool> attr_done[64];  // per device; zero-initialised (static storage)
@@ -498,13 +542,15 @@ cudaError_t launch_rows(const RowsParams &p, int rows, int C, const CUtensorMap 
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !attr_done[dev].load(std::memory_order_acquire)) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Layout<Page>::kSmem));
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) attr_done[dev].store(true, std::memory_order_release);  // setting twice is harmless
   }
+  const int slots = 148 * int(std::min<size_t>(227 * 1024 / (Layout<Page>::kSmem + 1024), 16));
+  const int C = cluster_size(rows, p.num_kv_heads, max_pages, Page::WARPS, slots);
+  if ((long long)rows * C > 0x7fffffffLL) return cudaErrorInvalidValue;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(rows) * C, p.num_kv_heads);
-  cfg.blockDim = dim3(kWarps * 32);
+  cfg.blockDim = dim3(Page::WARPS * 32);
   cfg.dynamicSmemBytes = Layout<Page>::kSmem;
   cfg.stream = stream;
   cudaLaunchAttribute at{};
@@ -517,21 +563,21 @@ cudaError_t launch_rows(const RowsParams &p, int rows, int C, const CUtensorMap 
 }
 
 template <class Page>
-cudaError_t launch_page(const RowsParams &p, int rows, int C, const CUtensorMap &km, const CUtensorMap &vm,
+cudaError_t launch_page(const RowsParams &p, int rows, int max_pages, const CUtensorMap &km, const CUtensorMap &vm,
                         cudaStream_t stream) {
-  return p.weight_sum ? launch_rows<Page, true>(p, rows, C, km, vm, stream)
-                      : launch_rows<Page, false>(p, rows, C, km, vm, stream);
+  return p.weight_sum ? launch_rows<Page, true>(p, rows, max_pages, km, vm, stream)
+                      : launch_rows<Page, false>(p, rows, max_pages, km, vm, stream);
 }
 
 template <int D>
-cudaError_t launch_f32(const RowsParams &p, int rows, int C, cudaStream_t stream) {
+cudaError_t launch_f32(const RowsParams &p, int rows, int max_pages, cudaStream_t stream) {
   const CUtensorMap none{};
   switch (p.group) {
-    case 1: return launch_page<PageF32<D, 1>>(p, rows, C, none, none, stream);
-    case 2: return launch_page<PageF32<D, 2>>(p, rows, C, none, none, stream);
-    case 4: return launch_page<PageF32<D, 4>>(p, rows, C, none, none, stream);
-    case 7: return launch_page<PageF32<D, 7>>(p, rows, C, none, none, stream);
-    case 8: return launch_page<PageF32<D, 8>>(p, rows, C, none, none, stream);
+    case 1: return launch_page<PageF32<D, 1>>(p, rows, max_pages, none, none, stream);
+    case 2: return launch_page<PageF32<D, 2>>(p, rows, max_pages, none, none, stream);
+    case 4: return launch_page<PageF32<D, 4>>(p, rows, max_pages, none, none, stream);
+    case 7: return launch_page<PageF32<D, 7>>(p, rows, max_pages, none, none, stream);
+    case 8: return launch_page<PageF32<D, 8>>(p, rows, max_pages, none, none, stream);
     default: return cudaErrorInvalidValue;
   }
 }
@@ -567,20 +613,19 @@ cudaError_t launch_checked(const WindowArgs &a, cudaStream_t stream) {
   // by the window where there is one, not by this call's contexts: a row's result does not
   // change with the longest context it is batched with
   const int64_t most = a.window > 0 ? int64_t(a.window) + a.sinks : a.max_ctx;
-  const int C = cluster_size(a.num_rows, a.num_kv_heads, int(std::min<int64_t>(most / kBS + 2, 1 << 26)));
-  if ((long long)a.num_rows * C > 0x7fffffffLL) return cudaErrorInvalidValue;
+  const int max_pages = int(std::min<int64_t>(most / kBS + 2, 1 << 26));
   if (a.dtype == MS_DTYPE_F32)
-    return a.head_dim == 128 ? launch_f32<128>(p, a.num_rows, C, stream) : launch_f32<64>(p, a.num_rows, C, stream);
+    return a.head_dim == 128 ? launch_f32<128>(p, a.num_rows, max_pages, stream) : launch_f32<64>(p, a.num_rows, max_pages, stream);
   CUtensorMap km, vm;
   const int64_t tiles = a.pool_blocks * a.num_kv_heads;
   if (!encode_pool_tensor_map(&km, a.k_pool, a.dtype, a.head_dim, tiles) ||
       !encode_pool_tensor_map(&vm, a.v_pool, a.dtype, a.head_dim, tiles))
     return cudaErrorInvalidValue;
   if (a.dtype == MS_DTYPE_BF16)
-    return a.head_dim == 128 ? launch_page<PageTc<__nv_bfloat16, 128, 3>>(p, a.num_rows, C, km, vm, stream)
-                             : launch_page<PageTc<__nv_bfloat16, 64, 4>>(p, a.num_rows, C, km, vm, stream);
-  return a.head_dim == 128 ? launch_page<PageTc<__half, 128, 3>>(p, a.num_rows, C, km, vm, stream)
-                           : launch_page<PageTc<__half, 64, 4>>(p, a.num_rows, C, km, vm, stream);
+    return a.head_dim == 128 ? launch_page<PageTc<__nv_bfloat16, 128>>(p, a.num_rows, max_pages, km, vm, stream)
+                             : launch_page<PageTc<__nv_bfloat16, 64>>(p, a.num_rows, max_pages, km, vm, stream);
+  return a.head_dim == 128 ? launch_page<PageTc<__half, 128>>(p, a.num_rows, max_pages, km, vm, stream)
+                           : launch_page<PageTc<__half, 64>>(p, a.num_rows, max_pages, km, vm, stream);
 }
 
 bool common_ok(const WindowArgs &a) {
