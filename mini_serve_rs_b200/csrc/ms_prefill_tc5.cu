@@ -171,6 +171,7 @@ struct Prefill5Params {
   int window, sinks;  // row at p sees j <= p with p - j < window or j < sinks
   int table_rows;
   int64_t pool_blocks;
+  int splits;  // CTAs of a cluster that share one tile's groups (grid z)
 };
 
 constexpr int kHalves = 2;  // query halves of 128 rows per CTA, sharing every K/V tile
@@ -310,14 +311,28 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
     dead1 = VisiblePages::lowest_key(pos0, p.window) + shift;
     dead0 = min(p.sinks, dead1);
   }
-  const int ngroups = (kv_len + kKeys - 1) / kKeys;
+  const int all_groups = (kv_len + kKeys - 1) / kKeys;
+  // windowed build: this CTA's share of the groups, [g0, g0 + ngroups); below, g counts from g0
+  int ngroups = all_groups, g0 = 0;
+  if constexpr (WIN) {
+    const int share = (all_groups + p.splits - 1) / p.splits;
+    g0 = min(int(blockIdx.z) * share, all_groups);
+    ngroups = min(share, all_groups - g0);
+  }
   const int ntiles = 2 * ngroups;  // ring order K0 V0 K1 V1 ...: K(g) is tile 2g, V(g) tile 2g + 1
   // groups each query half attends to (its last token's causal range); half 1 may be empty
   int ng[kHalves];
+  bool last_half0;  // half 0 attends to the tile's last group
 #pragma unroll
   for (int h = 0; h < kHalves; ++h) {
     const int last = min(nrows, (h + 1) * TPH);  // tokens up to the end of half h
     ng[h] = last > h * TPH ? (pos0 + last + shift + kKeys - 1) / kKeys : 0;
+  }
+  last_half0 = ng[0] == all_groups;
+  const bool last_half1 = ng[1] == all_groups;
+  if constexpr (WIN) {
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) ng[h] = min(max(ng[h] - g0, 0), ngroups);
   }
 
   if (t == 0) {
@@ -378,7 +393,7 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
     if (lane == 0) mbar_arrive(&q_full);
   }
 
-  float l_run = 0.f;
+  float l_run = 0.f, m_run = -INFINITY;
   if (warp < 4 * kHalves) {
     // ---- softmax: row rt of query half qh ----
     const uint32_t lane_off = uint32_t((warp & 3) * 32) << 16;
@@ -395,8 +410,7 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
     }
     const float c = p.qscale;
     // the lowest half that attends to the last group zeroes its V rows past the sequence
-    const bool zeroes_v = ng_q == ngroups && (qh == 0 || ng[0] < ngroups);
-    float m_run = -INFINITY;
+    const bool zeroes_v = qh == 0 ? last_half0 : last_half1 && !last_half0;
     for (int g = 0; g < ng_q; ++g) {
       if (!__all_sync(kFull, wait_or_abort(&s_full[qh], g & 1, &abort_s))) {
         abort_s = 1;
@@ -406,7 +420,7 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
       // S is read from TMEM twice, 32 columns at a time (the next chunk loads while one is used):
       // pass 1 takes the row max, pass 2 turns the scores into P.  Only groups that reach past
       // the half's first position take the causal mask (a CTA-uniform branch).
-      const int key0 = g * kKeys;
+      const int key0 = (g0 + g) * kKeys;
       const bool diag = key0 + kKeys - 1 > pos_first || (WIN && key0 < lo_last);
       constexpr int NC = kKeys / 32;
       // bits: windowed build, the visible keys of the 32-column chunk (one register instead of
@@ -507,7 +521,7 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
       // the last group's V rows past the sequence (stale, or pages never loaded) -> 0
       const int vk = kv_len - key0;
       int z0 = kKeys, z1 = kKeys;  // keys [z0, z1) of the group
-      if (zeroes_v && g == ngroups - 1 && vk < kKeys) z0 = vk;
+      if (zeroes_v && g0 + g == all_groups - 1 && vk < kKeys) z0 = vk;
       // windowed build: and the dead keys before the window (half 0 attends to every group they
       // reach, and its PV is issued first); where both meet in one group, in two rounds
       const int y0 = max(0, dead0 - key0), y1 = min(kKeys, dead1 - key0);
@@ -572,8 +586,8 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
         for (int kk = 0; kk < kKeys / 16; ++kk) umma_ts(d, a + kk * 8, b0 + uint64_t((kk * 2048) >> 4), id_o, kk > 0 ? 1u : acc0);
         umma_commit(&pv_done[h]);
       };
-      bool ok = wait_or_abort(&q_full, 0, &abort_s) && wait_tile(0);
-      if (ok) {
+      bool ok = wait_or_abort(&q_full, 0, &abort_s) && (ngroups == 0 || wait_tile(0));
+      if (ok && ngroups > 0) {
 #pragma unroll
         for (int h = 0; h < kHalves; ++h)
           if (ng[h] > 0) issue_s(h, 0);
@@ -629,8 +643,8 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
       }
       return table[i];
     };
-    int kw = 0, vw = 0;
-    int kcur = table_at(lane), vcur = kcur, knxt = table_at(32 + lane), vnxt = knxt;
+    int kw = g0 * PAGES >> 5, vw = kw;
+    int kcur = table_at(32 * kw + lane), vcur = kcur, knxt = table_at(32 * (kw + 1) + lane), vnxt = knxt;
     int issued = 0;
     for (int i = 0; i < ntiles; ++i) {
       const int slot = i % NSLOT;
@@ -639,7 +653,7 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
         break;
       }
       const bool is_v = i & 1;
-      const int grp = i >> 1;
+      const int grp = g0 + (i >> 1);
       const int first = grp * PAGES, n = min(PAGES, npages - first);
       const int w = first >> 5;
       int &cw = is_v ? vw : kw, &cur = is_v ? vcur : kcur, &nxt = is_v ? vnxt : knxt;
@@ -684,7 +698,70 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
   tc_fence_before();
   const bool all_ok = __syncthreads_and(ok_end);
   tc_fence_after();
-  if (all_ok) {
+  if (WIN && p.splits > 1) {
+    // Join the cluster's shares of the tile: each CTA leaves its rows' maxima, sums and
+    // unnormalised O (f32, 16-byte chunks XOR-swizzled by row) in its shared memory (the ring and
+    // the Q tile are free), then takes every splits-th run of rows of the tile.
+    float *ro = reinterpret_cast<float *>(ring);  // [2 x 128 rows][D]
+    float *rm = reinterpret_cast<float *>(sq), *rl = rm + kHalves * kRows;
+    constexpr int NCH = D / 4;  // 16-byte chunks per row
+    if (warp < 4 * kHalves) {
+      const int r = qh * kRows + rt;
+      rm[r] = all_ok ? m_run : NAN;  // a NaN tells the cluster that a wait ran out
+      rl[r] = l_run;
+      if (all_ok && ng_q > 0) {
+        const uint32_t tm_o = tmem + qh * 256 + kKeys + (uint32_t((warp & 3) * 32) << 16);
+#pragma unroll
+        for (int c0 = 0; c0 < D; c0 += 32) {
+          float o[32];
+          tmem_ld32(tm_o + c0, o);
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<float4 *>(ro + r * D + ((((c0 + i) >> 2) ^ (r % NCH)) << 2)) =
+                make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        }
+      }
+    }
+    if (!all_ok && t == 0) atomicOr(p.status, kStatusWaitTimeout);
+    cluster_sync();
+    // CPR threads per row, 8 values each; the CTA's rows 2 at a time per 2 * CPR threads
+    const int cc = t % CPR;
+    for (int r = int(blockIdx.z) + p.splits * (t / CPR); r < kHalves * kRows; r += p.splits * (kThreads5 / CPR)) {
+      const int tk = (r / kRows) * TPH + (r % kRows) / RPT, hd = r % RPT;
+      if (hd >= G || tk >= nrows) continue;
+      float M = -INFINITY, L = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      bool bad = false;
+      for (int s = 0; s < p.splits; ++s) {
+        const float m = peer_f32(rm + r, s);
+        bad |= m != m;
+        M = fmaxf(M, m);
+      }
+      for (int s = 0; s < p.splits; ++s) {
+        const float m = peer_f32(rm + r, s);
+        if (m == -INFINITY) continue;  // a share that saw nothing has not written its O
+        const float f = ex2_approx(m - M);
+        L += f * peer_f32(rl + r, s);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint4 u = peer_u4(reinterpret_cast<const uint32_t *>(ro + r * D + (((2 * cc + k) ^ (r % NCH)) << 2)), s);
+          o[4 * k] += f * __uint_as_float(u.x);
+          o[4 * k + 1] += f * __uint_as_float(u.y);
+          o[4 * k + 2] += f * __uint_as_float(u.z);
+          o[4 * k + 3] += f * __uint_as_float(u.w);
+        }
+      }
+      if (bad) continue;
+      const float inv = L > 0.f ? 1.f / L : 0.f;
+      uint4 w;
+      w.x = pack_pair<T>(o[0] * inv, o[1] * inv);
+      w.y = pack_pair<T>(o[2] * inv, o[3] * inv);
+      w.z = pack_pair<T>(o[4] * inv, o[5] * inv);
+      w.w = pack_pair<T>(o[6] * inv, o[7] * inv);
+      *reinterpret_cast<uint4 *>(static_cast<T *>(p.out) +
+                                 ((size_t(row0) + tk) * p.num_kv_heads * G + size_t(kvh) * G + hd) * D + cc * 8) = w;
+    }
+    cluster_sync();  // no CTA leaves while another may read its shared memory
+  } else if (all_ok) {
     if (warp < 4 * kHalves && ng_q > 0) {
       // O row / l -> shared memory (the Q tile is free once the MMAs drained): tile row
       // R = 32 warp + lane, D * 2 bytes, 16-byte chunk c at c ^ (R & 7); then this warp's 32
@@ -743,6 +820,20 @@ cudaError_t launch_t5(const Prefill5Params &p, int num_tiles, cudaStream_t strea
     attr_done[dev].store(true, std::memory_order_release);  // setting twice is harmless
   }
   if (num_tiles > 65535) return cudaErrorInvalidValue;
+  if constexpr (WIN) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(p.num_kv_heads, num_tiles, p.splits);
+    cfg.blockDim = dim3(kThreads5);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = at.val.clusterDim.y = 1;
+    at.val.clusterDim.z = p.splits;
+    cfg.attrs = &at;
+    cfg.numAttrs = p.splits > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kern, p);
+  }
   dim3 grid(p.num_kv_heads, num_tiles);
   kern<<<grid, kThreads5, smem, stream>>>(p);
   return cudaGetLastError();
@@ -770,6 +861,13 @@ cudaError_t t5_type(const Prefill5Params &p, int dtype, int head_dim, int group,
     if (head_dim == 64) return t5_group<__half, 64, WIN>(p, group, num_tiles, stream);
   }
   return cudaErrorInvalidValue;
+}
+
+// CTAs that share a tile: with fewer (tile, kv head) pairs than the 148 SMs hold (one CTA each),
+// the groups of a tile are split so that they fill one wave, at least 4 groups a CTA.
+int window_splits(long long pairs, int max_groups) {
+  const long long s = std::min<long long>(148 / std::max(1LL, pairs), max_groups / 4);
+  return int(std::max(1LL, std::min(8LL, s)));
 }
 
 }  // namespace
@@ -814,7 +912,12 @@ cudaError_t launch_window_prefill_tc5(const WindowArgs &a, cudaStream_t stream) 
   p.sinks = a.sinks;
   p.table_rows = a.table_rows;
   p.pool_blocks = a.pool_blocks;
-  return t5_type<true>(p, a.dtype, a.head_dim, a.num_heads / a.num_kv_heads, a.num_tiles, stream);
+  const int group = a.num_heads / a.num_kv_heads;
+  const int64_t keys = std::min<int64_t>(int64_t(a.max_blocks_per_seq) * kBS,
+                                         a.window > 0 ? int64_t(a.window) + a.sinks + prefill_tc5_tokens_per_tile(group)
+                                                      : int64_t(a.max_blocks_per_seq) * kBS);
+  p.splits = window_splits((long long)a.num_tiles * a.num_kv_heads, int(keys / kKeys));
+  return t5_type<true>(p, a.dtype, a.head_dim, group, a.num_tiles, stream);
 }
 
 }  // namespace attn

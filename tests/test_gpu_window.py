@@ -207,6 +207,29 @@ def test_chunks_every_head_layout(group, d):
         check(out, want, absv, smax, max(ctx), dt, exp_err=8e-5)
 
 
+@pytest.mark.parametrize("window,sinks", [(0, 0), (2500, 4), (2047, 130), (1100, 0)])
+@pytest.mark.parametrize("name,group,hkv,d", [("bf16", 2, 1, 128), ("f16", 1, 2, 64), ("bf16", 7, 2, 64)])
+def test_chunks_of_few_tiles_are_split(name, group, hkv, d, window, sinks):
+    """Few tiles share their keys among the CTAs of a cluster; a short one leaves some without any."""
+    dt = DTYPES[name]
+    chunks = [(3000, 90), (0, 5), (1500, 1)]
+    ctx = [s + n for s, n in chunks]
+    k, v, tables, rt = cache(ctx, [s for s, _ in chunks], window, sinks, hkv, d, dt, window)
+    T = sum(n for _, n in chunks)
+    q = (2 * torch.randn(T, hkv * group, d, generator=torch.Generator().manual_seed(6))).to(dt)
+    out = torch.full(q.shape, math.nan, dtype=dt, device=DEV)
+    tl = tiles_of(chunks, rt, group)
+    sync_ok(E.lib().ms_launch_window_prefill(ptr(q.to(DEV)), ptr(k.to(DEV)), ptr(v.to(DEV)), k.shape[0],
+                                             ptr(tables.to(DEV)), tables.shape[0], tables.shape[1], ptr(tl.to(DEV)),
+                                             len(tl), window, sinks, ptr(out), hkv * group, hkv, d, 16, ref.scale_of(d),
+                                             dt_code(q), None))
+    assert E.kernel_status(0) == 0
+    rows = [s + j + 1 for s, n in chunks for j in range(n)]
+    rrt = torch.tensor([int(rt[i]) for i, (s, n) in enumerate(chunks) for _ in range(n)])
+    want, _, absv, smax = want_rows(q, k, v, tables, rrt, rows, window, sinks)
+    check(out, want, absv, smax, max(ctx), dt, exp_err=8e-5)
+
+
 # ---- attention weights ------------------------------------------------------------
 
 def run_weights(q, k, v, tables, rt, ctx, out, w, max_ctx=None, ws=None, stream=None):
