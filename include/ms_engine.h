@@ -291,6 +291,15 @@ int ms_engine_profile_allreduce(ms_engine *eng, int64_t *calls, double *ms_total
 int ms_engine_set_graphs(ms_engine *eng, int32_t on);
 int ms_engine_graph_stats(const ms_engine *eng, int64_t *captures, int64_t *replays, int32_t *cached);
 
+/* Sliding-window attention (Qwen2's sliding_window / max_window_layers; the
+ * reference builds such a mask only for prompts).  In layers >= first_layer
+ * of later steps the token at position p attends to the keys j <= p with
+ * p - j < window or j < sinks (ms_launch_window_attention and
+ * ms_launch_window_prefill); window = 0 restores full attention.  Block
+ * tables still cover the whole sequence.  Drops the captured graphs; under
+ * tensor parallelism every rank makes the same call between the same steps. */
+int ms_engine_set_window(ms_engine *eng, int32_t window, int32_t sinks, int32_t first_layer);
+
 /* Tensor parallelism: *fused = 1 when the all-reduces after o_proj and
  * down_proj run as one peer-memory kernel fused with the residual add and
  * RMSNorm (NVLink, CUDA IPC mappings set up at creation), 0 when they go

@@ -20,6 +20,9 @@ class ModelConfig:
     qk_norm: bool = True
     attention_bias: bool = False
     tie_word_embeddings: bool = True
+    # keys a token attends to in layers >= max_window_layers; None: the whole context
+    sliding_window: Optional[int] = None
+    max_window_layers: int = 0
 
     def hd(self) -> int:
         return self.head_dim or self.hidden_size // self.num_attention_heads

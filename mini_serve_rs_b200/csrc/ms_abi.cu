@@ -213,6 +213,21 @@ extern "C" int ms_engine_set_tp_fused(ms_engine *eng, int32_t on) {
   return MS_OK;
 }
 
+extern "C" int ms_engine_set_window(ms_engine *eng, int32_t window, int32_t sinks, int32_t first_layer) {
+  if (!eng) return MS_E_INVALID;
+  if (eng->pending) return eng->fail(MS_E_INVALID, "ms_engine_set_window between launch and wait");
+  if (window < 0 || sinks < 0 || first_layer < 0 || first_layer > eng->L)
+    return eng->fail(MS_E_INVALID, "window and sinks must not be negative, first_layer within the layers");
+  if (window == eng->window && sinks == eng->window_sinks && first_layer == eng->window_layer0) return MS_OK;
+  cudaSetDevice(eng->dev);
+  cudaStreamSynchronize(eng->stream);
+  eng->drop_graphs();  // captured with the old window
+  eng->window = window;
+  eng->window_sinks = sinks;
+  eng->window_layer0 = first_layer;
+  return MS_OK;
+}
+
 extern "C" int ms_engine_set_graphs(ms_engine *eng, int32_t on) {
   if (!eng) return MS_E_INVALID;
   if (eng->pending) return eng->fail(MS_E_INVALID, "ms_engine_set_graphs between launch and wait");

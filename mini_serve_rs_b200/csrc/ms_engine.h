@@ -70,6 +70,10 @@ struct Engine {
   bool use_tc = false;
   std::vector<CUtensorMap> kmaps, vmaps;
 
+  // sliding window of layers >= window_layer0 (ms_engine_set_window); 0: full attention
+  int window = 0, window_sinks = 0, window_layer0 = 0;
+  bool windowed(int layer) const { return window > 0 && layer >= window_layer0; }
+
   // per-slot device state
   int32_t *d_block_tables = nullptr;  // [max_seqs][max_blocks_per_seq]
   int32_t *d_slot_last = nullptr;     // [max_seqs]
@@ -196,6 +200,7 @@ struct StepPlan {
   int max_ctx_dec = 0;
   long long blocks_dec = 0;  // sum over decode rows of pages read
   double ctx_dec = 0.0;      // sum over decode rows of keys read
+  double ctx_win = 0.0;      // the same in windowed layers
   bool split = false;        // decode rows via row list + prefill tiles
   // decode attention launch shape
   int part = 1;              // pages per split-K partition

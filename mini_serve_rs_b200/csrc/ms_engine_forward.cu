@@ -127,7 +127,46 @@ int enqueue_forward(Engine *eng, const StepPlan &plan) {
                                            eng->d_slots, eng->qbuf, kp, vp, T, eng->hq, eng->hkv, eng->D,
                                            eng->opts.block_size, eps, dt, st, eng->d_status));
     // paged attention: one-token rows through split-K decode, prompt chunks through prefill tiles
-    if (plan.n_dec > 0) {
+    // (windowed layers: K3w and K3pw)
+    WindowArgs wa{};
+    if (eng->windowed(l)) {
+      wa.q = eng->qbuf;
+      wa.k_pool = kp;
+      wa.v_pool = vp;
+      wa.pool_blocks = eng->opts.pool_blocks;
+      wa.block_tables = eng->d_block_tables;
+      wa.table_rows = eng->opts.max_seqs;
+      wa.max_blocks_per_seq = eng->opts.max_blocks_per_seq;
+      wa.window = eng->window;
+      wa.sinks = eng->window_sinks;
+      wa.out = eng->attn;
+      wa.num_heads = eng->hq;
+      wa.num_kv_heads = eng->hkv;
+      wa.head_dim = eng->D;
+      wa.block_size = eng->opts.block_size;
+      wa.scale = 1.0f / std::sqrt(float(eng->D));
+      wa.dtype = dt;
+      wa.status = eng->d_status;
+    }
+    if (plan.n_dec > 0 && eng->windowed(l)) {
+      WindowArgs a = wa;
+      a.row_table = eng->d_row_table;
+      a.row_ctx = eng->d_row_ctx;
+      a.row_index = dec_rows;
+      a.num_rows = plan.n_dec;
+      a.max_ctx = eng->opts.max_blocks_per_seq * eng->opts.block_size;
+      if (eng->use_tc) {
+        a.k_map = &eng->kmaps[l];
+        a.v_map = &eng->vmaps[l];
+      }
+      if (eng->profiling) MS_CUDA_TRY(prof_mark(eng));
+      MS_CUDA_TRY(launch_window_attention(a, st));
+      if (eng->profiling) {
+        MS_CUDA_TRY(prof_mark(eng));
+        eng->prof_bytes += plan.ctx_win * eng->hkv * eng->D * 2.0 * es + 2.0 * plan.n_dec * eng->hq * eng->D * es +
+                           plan.ctx_win / eng->opts.block_size * 4.0 + 4.0 * plan.n_dec;
+      }
+    } else if (plan.n_dec > 0) {
       AttnArgs a{};
       a.q = eng->qbuf;
       a.k_pool = kp;
@@ -164,7 +203,11 @@ int enqueue_forward(Engine *eng, const StepPlan &plan) {
                            double(plan.blocks_dec) * 4.0 + 4.0 * plan.n_dec;
       }
     }
-    if (plan.n_tiles > 0) {
+    if (plan.n_tiles > 0 && eng->windowed(l)) {
+      wa.tiles = tiles;
+      wa.num_tiles = plan.n_tiles;
+      MS_CUDA_TRY(launch_window_prefill(wa, st));
+    } else if (plan.n_tiles > 0) {
       PrefillArgs pf{};
       pf.q = eng->qbuf;
       pf.k_pool = kp;
@@ -258,6 +301,8 @@ int enqueue_forward(Engine *eng, const StepPlan &plan) {
     const int parts = plan.n_dec > 0 ? (max_blk + part - 1) / part : 0;
     const int attn_launches = (plan.n_dec > 0 ? 1 + (parts > 1 ? 1 : 0) : 0) + (plan.n_tiles > 0 ? 1 : 0);
     eng->last_launches = 3 + (plan.sample ? 1 : 0) + int64_t(eng->L) * (4 + attn_launches);
+    if (parts > 1)  // windowed layers need no partition merge
+      for (int l = 0; l < eng->L; ++l) eng->last_launches -= eng->windowed(l) ? 1 : 0;
     eng->kernel_launches += eng->last_launches;
   }
   MS_CUDA_TRY(cudaMemcpyAsync(eng->h_next, eng->d_next, size_t(S) * 4, cudaMemcpyDeviceToHost, st));

@@ -137,6 +137,11 @@ int step_launch_impl(Engine *eng, const ms_step_desc *desc) {
   int T = 0, nd = 0, max_ctx = 0;
   long long total_blocks = 0;
   double total_ctx = 0.0;  // sum over packed rows of the keys each row attends to
+  double total_win = 0.0;  // the same in windowed layers
+  auto win_keys = [&](int ctx) {  // keys that the row at position ctx - 1 sees there
+    const int low = eng->window > 0 ? std::max(0, ctx - eng->window) : 0;
+    return double(ctx - low + std::min(eng->window_sinks, low));
+  };
   for (RowPlan &r : plan) {
     const Seq &s = *r.seq;
     const int end = r.start + r.ntok;
@@ -148,6 +153,7 @@ int step_launch_impl(Engine *eng, const ms_step_desc *desc) {
     max_ctx = std::max(max_ctx, end);
     for (int j = 0; j < r.ntok; ++j) {
       total_ctx += double(r.start + j + 1);
+      total_win += win_keys(r.start + j + 1);
       total_blocks += (r.start + j + 1 + 15) / 16;
     }
   }
@@ -182,6 +188,7 @@ int step_launch_impl(Engine *eng, const ms_step_desc *desc) {
         sp.max_ctx_dec = std::max(sp.max_ctx_dec, end);
         sp.blocks_dec += (end + 15) / 16;
         sp.ctx_dec += double(end);
+        sp.ctx_win += win_keys(end);
       } else {
         prow0.push_back(row0);
         pntok.push_back(r.ntok);
@@ -204,6 +211,7 @@ int step_launch_impl(Engine *eng, const ms_step_desc *desc) {
     sp.max_ctx_dec = max_ctx;
     sp.blocks_dec = total_blocks;
     sp.ctx_dec = total_ctx;
+    sp.ctx_win = total_win;
   }
 
   // ---- decode attention launch shape ----

@@ -108,6 +108,9 @@ struct WindowArgs {
   float scale;
   int dtype;
   unsigned *status;          // null: the standalone status word
+  const int32_t *row_index = nullptr;  // launch row -> packed row of q, out, row_ctx, row_table; null -> identity
+  const void *k_map = nullptr;         // CUtensorMap of the pools (16-bit); null -> encoded per call
+  const void *v_map = nullptr;
 };
 cudaError_t launch_window_attention(const WindowArgs &a, cudaStream_t stream);
 cudaError_t launch_window_prefill(const WindowArgs &a, cudaStream_t stream);

@@ -44,7 +44,7 @@ constexpr int kMaxCluster = 8;
 
 struct RowsParams {
   const void *q, *k_pool, *v_pool;
-  const int32_t *block_tables, *row_table, *row_ctx;
+  const int32_t *block_tables, *row_table, *row_ctx, *row_index;
   void *out;
   float *weight_sum, *raw;  // K3a: accumulators; raw scores [rows][Hkv][G][ctx16]
   int64_t weight_stride;
@@ -330,7 +330,8 @@ __global__ void __launch_bounds__(Page::WARPS * 32)
       reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + Layout<Page>::kStages);
 
-  const int row = blockIdx.x / C, part = blockIdx.x % C;  // part = rank in the cluster
+  const int ri = blockIdx.x / C, part = blockIdx.x % C;  // part = rank in the cluster
+  const int row = p.row_index ? p.row_index[ri] : ri;
   const int kvh = blockIdx.y, G = p.group;
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
   const int ctx = p.row_ctx[row], trow = p.row_table ? p.row_table[row] : row;
@@ -590,6 +591,7 @@ cudaError_t launch_checked(const WindowArgs &a, cudaStream_t stream) {
   p.block_tables = a.block_tables;
   p.row_table = a.row_table;
   p.row_ctx = a.row_ctx;
+  p.row_index = a.row_index;
   p.out = a.out;
   p.weight_sum = a.weight_sum;
   p.raw = static_cast<float *>(a.workspace);
@@ -618,9 +620,13 @@ cudaError_t launch_checked(const WindowArgs &a, cudaStream_t stream) {
     return a.head_dim == 128 ? launch_f32<128>(p, a.num_rows, max_pages, stream) : launch_f32<64>(p, a.num_rows, max_pages, stream);
   CUtensorMap km, vm;
   const int64_t tiles = a.pool_blocks * a.num_kv_heads;
-  if (!encode_pool_tensor_map(&km, a.k_pool, a.dtype, a.head_dim, tiles) ||
-      !encode_pool_tensor_map(&vm, a.v_pool, a.dtype, a.head_dim, tiles))
+  if (a.k_map && a.v_map) {
+    km = *static_cast<const CUtensorMap *>(a.k_map);
+    vm = *static_cast<const CUtensorMap *>(a.v_map);
+  } else if (!encode_pool_tensor_map(&km, a.k_pool, a.dtype, a.head_dim, tiles) ||
+             !encode_pool_tensor_map(&vm, a.v_pool, a.dtype, a.head_dim, tiles)) {
     return cudaErrorInvalidValue;
+  }
   if (a.dtype == MS_DTYPE_BF16)
     return a.head_dim == 128 ? launch_page<PageTc<__nv_bfloat16, 128>>(p, a.num_rows, max_pages, km, vm, stream)
                              : launch_page<PageTc<__nv_bfloat16, 64>>(p, a.num_rows, max_pages, km, vm, stream);
@@ -643,7 +649,7 @@ cudaError_t launch_window_attention(const WindowArgs &a, cudaStream_t stream) {
   if (!common_ok(a) || !a.row_ctx || a.tiles || a.max_ctx > int64_t(a.max_blocks_per_seq) * attn::kBS ||
       (!a.row_table && a.table_rows < a.num_rows))
     return cudaErrorInvalidValue;
-  if (a.weight_sum && (a.weight_stride < a.max_ctx || !ptr16(a.workspace) ||
+  if (a.weight_sum && (a.row_index || a.weight_stride < a.max_ctx || !ptr16(a.workspace) ||
                        a.workspace_bytes < attention_weights_workspace_bytes(a.num_rows, a.num_heads, a.max_ctx)))
     return cudaErrorInvalidValue;
   return launch_checked(a, stream);

@@ -71,6 +71,7 @@ _SIGS = {
                            C.POINTER(C.c_double)], C.c_int),
     "ms_engine_profile_allreduce": ([_P, C.POINTER(C.c_int64), C.POINTER(C.c_double)], C.c_int),
     "ms_engine_set_graphs": ([_P, _I32], C.c_int),
+    "ms_engine_set_window": ([_P, _I32, _I32, _I32], C.c_int),
     "ms_engine_tp_fused": ([_P, C.POINTER(_I32)], C.c_int),
     "ms_engine_set_tp_fused": ([_P, _I32], C.c_int),
     "ms_engine_graph_stats": ([_P, C.POINTER(C.c_int64), C.POINTER(C.c_int64), C.POINTER(_I32)], C.c_int),
@@ -216,7 +217,8 @@ class Engine:
         """cfg: any object with the fields of oracle-style Config (vocab_size,
         hidden_size, intermediate_size, num_hidden_layers, num_attention_heads,
         num_key_value_heads, head_dim or hd(), max_position_embeddings,
-        rope_theta, rms_norm_eps, qk_norm, attention_bias, tie_word_embeddings)."""
+        rope_theta, rms_norm_eps, qk_norm, attention_bias, tie_word_embeddings);
+        where it has a sliding_window, layers from its max_window_layers on use it."""
         self.lib = lib()
         self.cfg = cfg
         hd = cfg.hd() if hasattr(cfg, "hd") else cfg.head_dim
@@ -236,6 +238,8 @@ class Engine:
         if rc != MS_OK:
             raise error_for(rc, "ms_engine_create: " + self._err(None))
         self.h = h
+        if getattr(cfg, "sliding_window", None):
+            self.set_window(cfg.sliding_window, 0, getattr(cfg, "max_window_layers", 0))
         self._out_tok = np.zeros(max_seqs, np.uint32)
         self._out_flags = np.zeros(max_seqs, np.uint8)
 
@@ -381,6 +385,11 @@ class Engine:
     def set_graphs(self, on: bool):
         """Replay pure-decode steps from captured CUDA graphs (default on)."""
         self._check(self.lib.ms_engine_set_graphs(self.h, 1 if on else 0), "set_graphs")
+
+    def set_window(self, window: int, sinks: int = 0, first_layer: int = 0):
+        """Later steps attend within `window` keys (and the first `sinks`) in
+        layers >= first_layer (ms_engine_set_window); 0: full attention."""
+        self._check(self.lib.ms_engine_set_window(self.h, window, sinks, first_layer), "set_window")
 
     def graph_stats(self):
         """(graphs captured, steps replayed, graphs cached)."""
