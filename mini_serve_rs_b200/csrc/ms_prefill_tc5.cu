@@ -44,7 +44,15 @@
 // tile sees, packed into one run of virtual keys (sink pages, then the
 // window's), so a few sinks do not cost a group of their own and the window
 // starts at a page, not at a group.  Groups that reach below the last row's
-// window or past the first row's position take the two-sided mask.
+// window or past the first row's position take the two-sided mask, as one
+// 32-bit word per 32 columns, and only in the chunks that a row of the warp
+// does not see whole.  With fewer (tile, kv head) pairs than SMs a cluster
+// shares a tile's groups and joins its rows over distributed shared memory.
+// Measured: 4 x 4096 tokens, window 2048, 16/8 heads of 128, bf16: 265 us, 0.47
+// of the floor at the measured bf16 rate (2.36 us per 128-key group of both
+// halves, as the causal build, and ~7 us of fixed cost per CTA, 6.9 waves);
+// 512 tokens behind 7680, window 4096: 82 us on 32 CTAs, 35 us split over 4 each,
+// of which the join takes 5 (its 96 KB per CTA come at ~14 B a cycle).
 //
 // Every wait is bounded (mbarrier polls that also watch a CTA abort flag);
 // on expiry the CTA records kStatusWaitTimeout, drains its MMAs and copies
@@ -287,8 +295,39 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
 
   const int kvh = blockIdx.x, tile = blockIdx.y;  // kv heads vary fastest: a tile's heads start together
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
-  const int row0 = p.tiles[tile * 4 + 0], nrows = p.tiles[tile * 4 + 1];
-  const int pos0 = p.tiles[tile * 4 + 2], trow = p.tiles[tile * 4 + 3];
+  int row0 = p.tiles[tile * 4 + 0], nrows = p.tiles[tile * 4 + 1];
+  int pos0 = p.tiles[tile * 4 + 2], trow = p.tiles[tile * 4 + 3];
+  // warp 8 sets up while the others fetch their first operands
+  if (t == 32 * 4 * kHalves) {
+    for (int i = 0; i < NSLOT; ++i) {
+      mbar_init(&full[i], 32);  // the copy warp's lanes
+      mbar_init(&empty[i], 1);
+    }
+    for (int h = 0; h < kHalves; ++h) {
+      mbar_init(&s_full[h], 1);
+      mbar_init(&p_ready[h], 4);  // one arrive per softmax warp of the half
+      mbar_init(&pv_done[h], 1);
+    }
+    mbar_init(&drain, 1);
+    mbar_init(&q_full, 4 * kHalves);  // one arrive per softmax warp once its Q rows are in shared memory
+    abort_s = 0;
+    mma_landed_s = 0;
+    issued_s = 0;
+    fence_barrier_init();
+  }
+  if (warp == 4 * kHalves) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base)),
+                 "r"(TMEM_COLS));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+  }
+  if constexpr (WIN) {
+    if (row0 < 0 || nrows < 0 || nrows > kHalves * TPH || pos0 < 0 || trow < 0 || trow >= p.table_rows ||
+        pos0 > p.max_blocks_per_seq * kBS - nrows) {
+      if (t == 0) atomicOr(p.status, kStatusBadIndex);
+      row0 = nrows = pos0 = trow = 0;  // an empty tile: nothing is loaded or stored
+    }
+    if (nrows == 0) pos0 = 0;
+  }
   const int32_t *table = p.block_tables + size_t(trow) * p.max_blocks_per_seq;
   int kv_len = pos0 + nrows;
   int npages = (kv_len + kBS - 1) / kBS;
@@ -298,12 +337,6 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
   [[maybe_unused]] VisiblePages vis;
   int shift = 0, dead0 = 0, dead1 = 0;
   if constexpr (WIN) {
-    if (row0 < 0 || nrows < 0 || nrows > kHalves * TPH || pos0 < 0 || trow < 0 || trow >= p.table_rows ||
-        pos0 > p.max_blocks_per_seq * kBS - nrows) {
-      if (t == 0) atomicOr(p.status, kStatusBadIndex);
-      return;
-    }
-    if (nrows == 0) return;
     vis = VisiblePages(pos0, kv_len, p.window, p.sinks);
     shift = vis.shift();
     npages = vis.count;
@@ -335,46 +368,31 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
     for (int h = 0; h < kHalves; ++h) ng[h] = min(max(ng[h] - g0, 0), ngroups);
   }
 
-  if (t == 0) {
-    for (int i = 0; i < NSLOT; ++i) {
-      mbar_init(&full[i], 32);  // the copy warp's lanes
-      mbar_init(&empty[i], 1);
-    }
-    for (int h = 0; h < kHalves; ++h) {
-      mbar_init(&s_full[h], 1);
-      mbar_init(&p_ready[h], 4);  // one arrive per softmax warp of the half
-      mbar_init(&pv_done[h], 1);
-    }
-    mbar_init(&drain, 1);
-    mbar_init(&q_full, 4 * kHalves);  // one arrive per softmax warp once its Q rows are in shared memory
-    abort_s = 0;
-    mma_landed_s = 0;
-    issued_s = 0;
-    fence_barrier_init();
-  }
-  if (warp == 0) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base)),
-                 "r"(TMEM_COLS));
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
-  }
   // softmax thread t: query half qh = warp / 4, row rt = t % 128 of that half (TMEM lane rt)
   const int qh = warp >> 2, rt = t & (kRows - 1);
   const int tok = qh * TPH + rt / RPT, head = rt % RPT;
   const bool rvalid = warp < 4 * kHalves && head < G && tok < nrows;
   const int ng_q = qh == 0 ? ng[0] : ng[1];  // groups of this thread's half (softmax warps)
-  // the CTA starts here: the copy warp's first K/V tiles overlap the Q load below
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = tmem_base;
   // Rows by whole lines: RPI rows of the tile per warp instruction, CPR lanes x 16 bytes each.
   // Softmax warp w owns tile rows [32 w, 32 w + 32) (its TMEM lanes), so it loads Q and
   // stores O for exactly those rows.
   constexpr int CPR = D / 8, RPI = 32 / CPR;
+  uint4 qv[32 / RPI];
+  auto table_at = [&](int i) {
+    if (i >= npages) return 0;
+    if constexpr (WIN) {
+      const int page = table[vis.page_at(i)];
+      if (page >= 0 && page < p.pool_blocks) return page;
+      atomicOr(p.status, kStatusBadIndex);
+      return 0;
+    }
+    return table[i];
+  };
+  const int first_window = g0 * PAGES >> 5;  // of 32 page ids (copy warp)
+  int kcur = 0, knxt = 0;
   if (warp < 4 * kHalves) {
-    // Q rows -> K-major swizzled tile (zeros for padding rows), all loads before the stores
+    // Q rows (zeros for padding rows): on their way while warp 8 sets up
     const int cc = lane % CPR, sub = lane / CPR;
-    uint4 qv[32 / RPI];
 #pragma unroll
     for (int i = 0; i < 32 / RPI; ++i) {
       const int r = (warp & 3) * 32 + i * RPI + sub;  // row within the half
@@ -383,6 +401,17 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
                      ((size_t(row0) + tk) * p.num_kv_heads * G + size_t(kvh) * G + hd) * D + cc * 8;
       qv[i] = hd < G && tk < nrows ? __ldg(reinterpret_cast<const uint4 *>(src)) : make_uint4(0, 0, 0, 0);
     }
+  } else if (warp > 4 * kHalves) {
+    kcur = table_at(32 * first_window + lane);
+    knxt = table_at(32 * (first_window + 1) + lane);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base;
+  if (warp < 4 * kHalves) {
+    // Q -> K-major swizzled tile
+    const int cc = lane % CPR, sub = lane / CPR;
 #pragma unroll
     for (int i = 0; i < 32 / RPI; ++i) {
       const int r = (warp & 3) * 32 + i * RPI + sub, dh = cc >> 3, c = cc & 7;
@@ -450,9 +479,18 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
           const uint32_t *cur = (k & 1) ? cb : ca;
           if (k + 1 < NC) tmem_ld32_async(tm_s + lane_off + 32 * (k + 1), (k & 1) ? ca : cb);
           const uint32_t bits = visible_bits(masked, k);
+          auto chunk_max = [&](auto m) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            mx[i & 3] = max3f(mx[i & 3], score(masked, cur, k, 2 * i, bits), score(masked, cur, k, 2 * i + 1, bits));
+            for (int i = 0; i < 16; ++i)
+              mx[i & 3] = max3f(mx[i & 3], score(m, cur, k, 2 * i, bits), score(m, cur, k, 2 * i + 1, bits));
+          };
+          // a masked group's chunks are mostly seen whole by a warp's rows: no select for those
+          if constexpr (WIN && decltype(masked)::value) {
+            if (__all_sync(kFull, bits == 0xffffffffu)) chunk_max(std::false_type{});
+            else chunk_max(masked);
+          } else {
+            chunk_max(masked);
+          }
         }
         return fmaxf(max3f(mx[0], mx[1], mx[2]), mx[3]);
       };
@@ -495,20 +533,29 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
           if (k + 1 < NC) tmem_ld32_async(tm_s + lane_off + 32 * (k + 1), (k & 1) ? ca : cb);
           const uint32_t bits = visible_bits(masked, k);
           uint32_t pk[16];
+          auto chunk_p = [&](auto m) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float x0, x1, a, b;
-            ffma2(x0, x1, score(masked, cur, k, 2 * i, bits), score(masked, cur, k, 2 * i + 1, bits), c, negm);
-            // (the polynomial gives 1e-38 for a masked score: the windowed build, whose masked V
-            // rows may be another row's live ones, keeps masked groups on ex2 and its exact 0)
-            if ((i & 7) < kExp2OnFma && !(WIN && decltype(masked)::value)) {  // a share of the exponentials off the transcendental unit
-              exp2_poly2(a, b, x0, x1);
-            } else {
-              a = ex2_approx(x0);
-              b = ex2_approx(x1);
+            for (int i = 0; i < 16; ++i) {
+              float x0, x1, a, b;
+              ffma2(x0, x1, score(m, cur, k, 2 * i, bits), score(m, cur, k, 2 * i + 1, bits), c, negm);
+              // a share of the exponentials off the transcendental unit (the polynomial gives 1e-38
+              // for a masked score: the windowed build, whose masked V rows may be another row's
+              // live ones, takes the exact 0 of ex2 where it masks)
+              if ((i & 7) < kExp2OnFma && !(WIN && decltype(m)::value)) {
+                exp2_poly2(a, b, x0, x1);
+              } else {
+                a = ex2_approx(x0);
+                b = ex2_approx(x1);
+              }
+              fadd2(ps[2 * (i & 3)], ps[2 * (i & 3) + 1], a, b);
+              pk[i] = pack_pair<T>(a, b);
             }
-            fadd2(ps[2 * (i & 3)], ps[2 * (i & 3) + 1], a, b);
-            pk[i] = pack_pair<T>(a, b);
+          };
+          if constexpr (WIN && decltype(masked)::value) {
+            if (__all_sync(kFull, bits == 0xffffffffu)) chunk_p(std::false_type{});
+            else chunk_p(masked);
+          } else {
+            chunk_p(masked);
           }
           tmem_st16u_async(tm_s + lane_off + 16 * k, pk);  // over S columns this thread has read
         }
@@ -633,18 +680,8 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
     // visible to the tensor core (fence.proxy.async) after its wait.
     constexpr int CPR = D / 8, RPI = 32 / CPR, IPP = kBS / RPI;  // chunks per row, rows per instruction, per page
     const int cc = lane % CPR, dh = cc >> 3, ch = cc & 7, r0 = lane / CPR;
-    auto table_at = [&](int i) {
-      if (i >= npages) return 0;
-      if constexpr (WIN) {
-        const int page = table[vis.page_at(i)];
-        if (page >= 0 && page < p.pool_blocks) return page;
-        atomicOr(p.status, kStatusBadIndex);
-        return 0;
-      }
-      return table[i];
-    };
-    int kw = g0 * PAGES >> 5, vw = kw;
-    int kcur = table_at(32 * kw + lane), vcur = kcur, knxt = table_at(32 * (kw + 1) + lane), vnxt = knxt;
+    int kw = first_window, vw = kw;
+    int vcur = kcur, vnxt = knxt;
     int issued = 0;
     for (int i = 0; i < ntiles; ++i) {
       const int slot = i % NSLOT;
@@ -724,41 +761,69 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
     }
     if (!all_ok && t == 0) atomicOr(p.status, kStatusWaitTimeout);
     cluster_sync();
-    // CPR threads per row, 8 values each; the CTA's rows 2 at a time per 2 * CPR threads
-    const int cc = t % CPR;
-    for (int r = int(blockIdx.z) + p.splits * (t / CPR); r < kHalves * kRows; r += p.splits * (kThreads5 / CPR)) {
-      const int tk = (r / kRows) * TPH + (r % kRows) / RPT, hd = r % RPT;
-      if (hd >= G || tk >= nrows) continue;
-      float M = -INFINITY, L = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    // weights of the shares, once per row: 2^(m_s - M) / L, 0 for a share that saw nothing
+    float *rw = rl + kHalves * kRows;  // [8][256], this CTA's rows by their place among them
+    for (int i = t; int(blockIdx.z) + p.splits * i < kHalves * kRows; i += kThreads5) {
+      const int r = int(blockIdx.z) + p.splits * i;
+      float m[8], l[8], M = -INFINITY, L = 0.f;
       bool bad = false;
-      for (int s = 0; s < p.splits; ++s) {
-        const float m = peer_f32(rm + r, s);
-        bad |= m != m;
-        M = fmaxf(M, m);
-      }
-      for (int s = 0; s < p.splits; ++s) {
-        const float m = peer_f32(rm + r, s);
-        if (m == -INFINITY) continue;  // a share that saw nothing has not written its O
-        const float f = ex2_approx(m - M);
-        L += f * peer_f32(rl + r, s);
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const uint4 u = peer_u4(reinterpret_cast<const uint32_t *>(ro + r * D + (((2 * cc + k) ^ (r % NCH)) << 2)), s);
-          o[4 * k] += f * __uint_as_float(u.x);
-          o[4 * k + 1] += f * __uint_as_float(u.y);
-          o[4 * k + 2] += f * __uint_as_float(u.z);
-          o[4 * k + 3] += f * __uint_as_float(u.w);
-        }
+      for (int s = 0; s < 8; ++s) {
+        m[s] = s < p.splits ? peer_f32(rm + r, s) : -INFINITY;
+        l[s] = s < p.splits ? peer_f32(rl + r, s) : 0.f;
       }
-      if (bad) continue;
-      const float inv = L > 0.f ? 1.f / L : 0.f;
-      uint4 w;
-      w.x = pack_pair<T>(o[0] * inv, o[1] * inv);
-      w.y = pack_pair<T>(o[2] * inv, o[3] * inv);
-      w.z = pack_pair<T>(o[4] * inv, o[5] * inv);
-      w.w = pack_pair<T>(o[6] * inv, o[7] * inv);
-      *reinterpret_cast<uint4 *>(static_cast<T *>(p.out) +
-                                 ((size_t(row0) + tk) * p.num_kv_heads * G + size_t(kvh) * G + hd) * D + cc * 8) = w;
+#pragma unroll
+      for (int s = 0; s < 8; ++s) {
+        bad |= m[s] != m[s];
+        M = fmaxf(M, m[s]);
+      }
+#pragma unroll
+      for (int s = 0; s < 8; ++s) {
+        m[s] = m[s] == -INFINITY ? 0.f : ex2_approx(m[s] - M);
+        L += m[s] * l[s];
+      }
+      const float inv = bad ? NAN : L > 0.f ? 1.f / L : 0.f;
+#pragma unroll
+      for (int s = 0; s < 8; ++s)
+        if (s < p.splits) rw[s * 256 + i] = m[s] == 0.f && !bad ? 0.f : m[s] * inv;
+    }
+    __syncthreads();
+    // A thread per 16-byte chunk of a row (whole rows per request, no bank conflicts), the chunks
+    // of every share and of two rows under way before the first is used (a share that saw nothing
+    // has not written its O: it is read and not used)
+    const int ch = t % NCH;
+    constexpr int RSTEP = kThreads5 / NCH, NR = 2;
+    const int mine = (kHalves * kRows - int(blockIdx.z) + p.splits - 1) / p.splits;  // rows of this CTA
+    for (int i0 = t / NCH; i0 < mine; i0 += NR * RSTEP) {
+      uint4 u[NR][8];
+#pragma unroll
+      for (int j = 0; j < NR; ++j) {
+        const int r = int(blockIdx.z) + p.splits * (i0 + j * RSTEP);
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+          if (s < p.splits && i0 + j * RSTEP < mine)
+            u[j][s] = peer_u4(reinterpret_cast<const uint32_t *>(ro + r * D + ((ch ^ (r % NCH)) << 2)), s);
+      }
+#pragma unroll
+      for (int j = 0; j < NR; ++j) {
+        const int i = i0 + j * RSTEP, r = int(blockIdx.z) + p.splits * i;
+        const int tk = (r / kRows) * TPH + (r % kRows) / RPT, hd = r % RPT;
+        if (i >= mine || hd >= G || tk >= nrows) continue;
+        float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+          const float f = s < p.splits ? rw[s * 256 + i] : 0.f;
+          if (f == 0.f) continue;
+          o[0] += f * __uint_as_float(u[j][s].x);
+          o[1] += f * __uint_as_float(u[j][s].y);
+          o[2] += f * __uint_as_float(u[j][s].z);
+          o[3] += f * __uint_as_float(u[j][s].w);
+        }
+        if (rw[i] != rw[i]) continue;  // a wait ran out
+        *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) +
+                                   ((size_t(row0) + tk) * p.num_kv_heads * G + size_t(kvh) * G + hd) * D + ch * 4) =
+            make_uint2(pack_pair<T>(o[0], o[1]), pack_pair<T>(o[2], o[3]));
+      }
     }
     cluster_sync();  // no CTA leaves while another may read its shared memory
   } else if (all_ok) {
@@ -804,7 +869,7 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS));
+  if (warp == 4 * kHalves) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS));
 }
 
 template <typename T, int D, int G, bool WIN>
