@@ -788,42 +788,32 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
         if (s < p.splits) rw[s * 256 + i] = m[s] == 0.f && !bad ? 0.f : m[s] * inv;
     }
     __syncthreads();
-    // A thread per 16-byte chunk of a row (whole rows per request, no bank conflicts), the chunks
-    // of every share and of two rows under way before the first is used (a share that saw nothing
-    // has not written its O: it is read and not used)
+    // A thread per 16-byte chunk of a row (whole rows per request, no bank conflicts), every
+    // share's chunk under way before the first is used (a share that saw nothing has not written
+    // its O: it is read and not used)
     const int ch = t % NCH;
-    constexpr int RSTEP = kThreads5 / NCH, NR = 2;
-    const int mine = (kHalves * kRows - int(blockIdx.z) + p.splits - 1) / p.splits;  // rows of this CTA
-    for (int i0 = t / NCH; i0 < mine; i0 += NR * RSTEP) {
-      uint4 u[NR][8];
+    for (int i = t / NCH; int(blockIdx.z) + p.splits * i < kHalves * kRows; i += kThreads5 / NCH) {
+      const int r = int(blockIdx.z) + p.splits * i;
+      const int tk = (r / kRows) * TPH + (r % kRows) / RPT, hd = r % RPT;
+      if (hd >= G || tk >= nrows) continue;
+      uint4 u[8];
 #pragma unroll
-      for (int j = 0; j < NR; ++j) {
-        const int r = int(blockIdx.z) + p.splits * (i0 + j * RSTEP);
+      for (int s = 0; s < 8; ++s)
+        if (s < p.splits) u[s] = peer_u4(reinterpret_cast<const uint32_t *>(ro + r * D + ((ch ^ (r % NCH)) << 2)), s);
+      float o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int s = 0; s < 8; ++s)
-          if (s < p.splits && i0 + j * RSTEP < mine)
-            u[j][s] = peer_u4(reinterpret_cast<const uint32_t *>(ro + r * D + ((ch ^ (r % NCH)) << 2)), s);
+      for (int s = 0; s < 8; ++s) {
+        const float f = s < p.splits ? rw[s * 256 + i] : 0.f;
+        if (f == 0.f) continue;
+        o[0] += f * __uint_as_float(u[s].x);
+        o[1] += f * __uint_as_float(u[s].y);
+        o[2] += f * __uint_as_float(u[s].z);
+        o[3] += f * __uint_as_float(u[s].w);
       }
-#pragma unroll
-      for (int j = 0; j < NR; ++j) {
-        const int i = i0 + j * RSTEP, r = int(blockIdx.z) + p.splits * i;
-        const int tk = (r / kRows) * TPH + (r % kRows) / RPT, hd = r % RPT;
-        if (i >= mine || hd >= G || tk >= nrows) continue;
-        float o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int s = 0; s < 8; ++s) {
-          const float f = s < p.splits ? rw[s * 256 + i] : 0.f;
-          if (f == 0.f) continue;
-          o[0] += f * __uint_as_float(u[j][s].x);
-          o[1] += f * __uint_as_float(u[j][s].y);
-          o[2] += f * __uint_as_float(u[j][s].z);
-          o[3] += f * __uint_as_float(u[j][s].w);
-        }
-        if (rw[i] != rw[i]) continue;  // a wait ran out
-        *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) +
-                                   ((size_t(row0) + tk) * p.num_kv_heads * G + size_t(kvh) * G + hd) * D + ch * 4) =
-            make_uint2(pack_pair<T>(o[0], o[1]), pack_pair<T>(o[2], o[3]));
-      }
+      if (rw[i] != rw[i]) continue;  // a wait ran out
+      *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) +
+                                 ((size_t(row0) + tk) * p.num_kv_heads * G + size_t(kvh) * G + hd) * D + ch * 4) =
+          make_uint2(pack_pair<T>(o[0], o[1]), pack_pair<T>(o[2], o[3]));
     }
     cluster_sync();  // no CTA leaves while another may read its shared memory
   } else if (all_ok) {
