@@ -412,10 +412,10 @@ __global__ void __launch_bounds__(Page::WARPS * 32)
   }
 
   // ---- merge the warps (the stages are free), then the cluster's CTAs ----
-  float *wo = reinterpret_cast<float *>(smem);         // [W][G][D]
-  float *wm = wo + W * kMaxGroup * D;             // [W][kMaxGroup] maxima, then sums
-  float *wl = wm + W * kMaxGroup;
-  float *co = wl + W * kMaxGroup;                 // the CTA's [G][D], maxima, sums
+  float *wo = reinterpret_cast<float *>(smem);         // [W][kMaxGroup][D]
+  float *wm = wo + W * kMaxGroup * D;                  // [W][kMaxGroup] maxima, then the row's
+  float *wl = wm + W * kMaxGroup;                      // and sums, then the row's reciprocal
+  float *co = wl + W * kMaxGroup;                      // the CTA's [G][D], maxima, sums
   float *cm = co + kMaxGroup * D, *cl = cm + kMaxGroup;
   const bool any_failed = __syncthreads_or(failed ? 1 : 0) != 0;
   pg.store(wo + warp * kMaxGroup * D, wm + warp * kMaxGroup, wl + warp * kMaxGroup, G);
@@ -439,49 +439,63 @@ __global__ void __launch_bounds__(Page::WARPS * 32)
       cl[h] = L;
     }
   }
+  // All CTAs' maxima and sums, one load a thread; then each head's maximum and the CTAs' factors
+  // 2^(m_c - M) / L (the warps' O is free by now).
+  float *tm = wo, *tl = tm + kMaxCluster * kMaxGroup, *tf = tl + kMaxCluster * kMaxGroup;  // [CTA][kMaxGroup]
   if (C > 1) {
-    cluster_arrive();
-    cluster_wait();
-    for (int i = part * W * 32 + t; i < G * D; i += C * W * 32) {
-      const int h = i / D;
-      float M = -INFINITY, L = 0.f, O = 0.f;
-      bool bad = false;
-      for (int c = 0; c < C; ++c) {
-        const float mc = peer_f32(cm + h, c);
-        bad |= mc != mc;
-        M = fmaxf(M, mc);
+    cluster_sync();
+    for (int i = t; i < C * kMaxGroup; i += W * 32) {
+      const int c = i / kMaxGroup, h = i % kMaxGroup;
+      if (h < G) {
+        tm[i] = peer_f32(cm + h, c);
+        tl[i] = peer_f32(cl + h, c);
       }
-      for (int c = 0; c < C; ++c) {
-        const float mc = peer_f32(cm + h, c), f = mc == -INFINITY ? 0.f : exp2f(mc - M);
-        L += f * peer_f32(cl + h, c);
-        O += f * peer_f32(co + i, c);
-      }
-      if (!bad) out[i] = Elem<T>::from_f(L > 0.f ? O / L : 0.f);
+    }
+  } else if (WEIGHTS) {
+    __syncthreads();
+    if (t < G) {
+      tm[t] = cm[t];
+      tl[t] = cl[t];
     }
   }
-  if constexpr (WEIGHTS) {
+  if (C > 1 || WEIGHTS) {
     __syncthreads();
-    if (t < G) {  // the row's maximum and reciprocal sum (the warps' slots are free)
+    if (t < G) {
       float M = -INFINITY, L = 0.f;
       bool bad = false;
       for (int c = 0; c < C; ++c) {
-        const float mc = C > 1 ? peer_f32(cm + t, c) : cm[t];
+        const float mc = tm[c * kMaxGroup + t];
         bad |= mc != mc;
         M = fmaxf(M, mc);
       }
       for (int c = 0; c < C; ++c) {
-        const float mc = C > 1 ? peer_f32(cm + t, c) : cm[t];
-        L += mc == -INFINITY ? 0.f : exp2f(mc - M) * (C > 1 ? peer_f32(cl + t, c) : cl[t]);
+        const float mc = tm[c * kMaxGroup + t], f = mc == -INFINITY ? 0.f : exp2f(mc - M);
+        tf[c * kMaxGroup + t] = f;
+        L += f * tl[c * kMaxGroup + t];
       }
       wm[t] = bad ? NAN : M;
       wl[t] = L > 0.f ? 1.f / L : 0.f;
     }
     __syncthreads();
-    if (C > 1) cluster_arrive();
+  }
+  const bool good = (C == 1 && !WEIGHTS) || wm[0] == wm[0];
+  if (C > 1 && good)
+    for (int i = part * W * 32 + t; i < G * D; i += C * W * 32) {
+      const int h = i / D;
+      float o[kMaxCluster], O = 0.f;
+#pragma unroll
+      for (int c = 0; c < kMaxCluster; ++c) o[c] = c < C ? peer_f32(co + i, c) : 0.f;
+#pragma unroll
+      for (int c = 0; c < kMaxCluster; ++c)
+        if (c < C) O += tf[c * kMaxGroup + h] * o[c];
+      out[i] = Elem<T>::from_f(O * wl[h]);
+    }
+  if (C > 1) cluster_arrive();
+  if constexpr (WEIGHTS) {
     float *sum = p.weight_sum + (size_t(trow) * p.num_kv_heads + kvh) * p.weight_stride;
     // 4 keys a thread, all heads' scores and the sums under way together: the CTA streams nothing
     // meanwhile (a key at a time this phase took a fifth of the kernel)
-    const int end = wm[0] == wm[0] ? min(b1 * kBS, ctx) : 0;
+    const int end = good ? min(b1 * kBS, ctx) : 0;
     const bool vec = (reinterpret_cast<uintptr_t>(sum) & 15) == 0;
     for (int key = b0 * kBS + 4 * t; key < end; key += 4 * W * 32) {
       float4 r[kMaxGroup];
@@ -516,8 +530,6 @@ __global__ void __launch_bounds__(Page::WARPS * 32)
           if (key + i < end) sum[key + i] = s[i];
       }
     }
-  } else {
-    if (C > 1) cluster_arrive();
   }
   if (C > 1) cluster_wait();  // no CTA leaves while another may read its shared memory
 }
