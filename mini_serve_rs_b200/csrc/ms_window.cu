@@ -22,7 +22,9 @@
 //    below one tcgen05 tile), online softmax in base 2 on the four scores a
 //    lane holds;
 //  * f32: a lane owns D / 32 dims; partial dot products of 16 tokens are
-//    reduced across the warp by a transposed butterfly.
+//    reduced across the warp by a transposed butterfly.  ~2000 cycles a page,
+//    so many warps with one 16 KB stage each do better than few with two (24
+//    rows, window 1001: 12 warps an SM 29.8 us, 6 warps 35.3).
 // The warps merge in shared memory, the CTAs of the cluster read one another's
 // maxima, sums and outputs there (distributed shared memory): one launch, no
 // workspace, and the split depends on the call's shape only, so equal calls
@@ -178,7 +180,7 @@ template <typename T_, int D_> struct PageTc {
 // ---- one page of one kv head: f32 on the FMA pipe ---------------------------------------
 template <int D_, int G> struct PageF32 {
   using T = float;
-  static constexpr int D = D_, WARPS = 2, NSTAGE = D == 128 ? 2 : 3;
+  static constexpr int D = D_, WARPS = 4, NSTAGE = D == 128 ? 1 : 2;
   static constexpr int DPL = D / 32, TILE = kBS * D, TILE_BYTES = TILE * 4;
   static constexpr int SUB = (G > 4) ? 8 : 16;  // tokens per scoring sub-tile
   static constexpr int NV = G * SUB, NVP = ((NV + 31) / 32) * 32;
