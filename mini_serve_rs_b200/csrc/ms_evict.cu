@@ -57,6 +57,7 @@ struct EvictParams {
   int64_t stride;
   int num_kv_heads;
   int chunks;      // 16-byte pieces of one K (V) row
+  int vec;         // weights and positions may be read and written 16 bytes at a time
   int32_t *lists;  // [rows][kv heads][2][half]: holes, movers
   int half;
   int32_t *moves;  // [rows][kv heads]: their number
@@ -249,24 +250,47 @@ __global__ void __launch_bounds__(NT, 1024 / NT) evict_kernel(EvictParams p, int
   }
 
   // ---- 1. the keep-th largest key ----
-  constexpr int U = 8;  // loads of U slots per thread before the first is used
-  for (int j0 = s0 + t; j0 < s1; j0 += U * NT) {
-    float w[U];
-    int pos[U];
+  // Slots go four to a thread here and in the last step, as vectors where the arrays allow it
+  // (p.vec; a slot index is a multiple of 4 and the stride too, so a vector never leaves its row),
+  // U of them under way before the first is used: these two steps are loads' latency.
+  constexpr int U = 3;
+  auto load_weights = [&](int j, float (&w)[4]) {
+    if (p.vec) {
+      Vec4<float>::load(w_in + j, w);
+    } else {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int j = j0 + u * NT;
-      w[u] = j < s1 ? w_in[j] : 0.f;
-      pos[u] = j < s1 ? position(j) : 0;
+      for (int i = 0; i < 4; ++i) w[i] = j + i < s1 ? w_in[j + i] : 0.f;
     }
+  };
+  auto load_positions = [&](int j, int (&pos)[4]) {
+    if (p.vec && j + 4 <= known) {
+      const int4 v = *reinterpret_cast<const int4 *>(pos_in + j);
+      pos[0] = v.x, pos[1] = v.y, pos[2] = v.z, pos[3] = v.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pos[i] = j + i < s1 ? position(j + i) : 0;
+    }
+  };
+  for (int j0 = s0 + 4 * t; j0 < s1; j0 += U * 4 * NT) {
+    float w[U][4];
+    int pos[U][4];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (j0 + u * 4 * NT < s1) {
+        load_weights(j0 + u * 4 * NT, w[u]);
+        load_positions(j0 + u * 4 * NT, pos[u]);
+      }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int j = j0 + u * NT;
-      if (j < s1) {
-        const uint32_t key = pos[u] < p.sinks || pos[u] >= next - p.recent ? 0xffffffffu : rank_key(w[u]);
-        keys[j - s0] = key;
-        atomicAdd(&sh.hist[0][key >> 21], 1u);
+      const int j = j0 + u * 4 * NT;
+      if (j >= s1) break;
+      uint32_t key[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        key[i] = pos[u][i] < p.sinks || pos[u][i] >= next - p.recent ? 0xffffffffu : rank_key(w[u][i]);
+        if (j + i < s1) atomicAdd(&sh.hist[0][key[i] >> 21], 1u);
       }
+      *reinterpret_cast<uint4 *>(keys + j - s0) = make_uint4(key[0], key[1], key[2], key[3]);  // (seg: a multiple of 32)
     }
   }
   uint32_t T = 0;
@@ -357,32 +381,46 @@ __global__ void __launch_bounds__(NT, 1024 / NT) evict_kernel(EvictParams p, int
   __syncthreads();
   // the lists, and the weights and positions of the slots that do not move
   const bool same_w = p.w_in == p.w_out, same_pos = p.pos_in == p.pos_out;
-  constexpr int V = 6;  // weights of V slots per thread under way at once
-  for (int j0 = s0 + t; j0 < s1; j0 += V * NT) {
-    float w[V];
-    int pos[V];
+  for (int j0 = s0 + 4 * t; j0 < s1; j0 += U * 4 * NT) {
+    float w[U][4];
+    int pos[U][4];
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const int j = j0 + v * NT;
-      const bool in_place = j < min(p.keep, s1) && (stay[(j - s0) >> 5] >> (j & 31) & 1);  // s0 is a multiple of 32
-      w[v] = in_place && !same_w ? w_in[j] : 0.f;
-      pos[v] = in_place && !(same_pos && j < known) ? position(j) : 0;
+    for (int u = 0; u < U; ++u) {
+      const int j = j0 + u * 4 * NT;
+      if (j < min(p.keep, s1)) {
+        if (!same_w) load_weights(j, w[u]);
+        load_positions(j, pos[u]);
+      }
     }
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const int j = j0 + v * NT, i = (j - s0) >> 5;
+    for (int u = 0; u < U; ++u) {
+      const int j = j0 + u * 4 * NT, i = (j - s0) >> 5;
       if (j >= s1) break;
-      const uint32_t s = stay[i], bit = 1u << (j & 31);
-      if (j < p.keep) {
-        if (s & bit) {
-          if (!same_w) w_out[j] = w[v];
-          if (!(same_pos && j < known)) pos_out[j] = pos[v];
-        } else {
-          holes[hole0[i] + __popc(~s & (bit - 1))] = j;
-        }
+      const uint32_t s = stay[i];  // s0 is a multiple of 32
+      const int b = j & 31;
+      // holes and movers are written again by their moves, which come later
+      if (p.vec && j + 4 <= min(p.keep, s1)) {
+        if (!same_w) Vec4<float>::store(w_out + j, w[u]);
+        if (!(same_pos && j + 4 <= known))
+          *reinterpret_cast<int4 *>(pos_out + j) = make_int4(pos[u][0], pos[u][1], pos[u][2], pos[u][3]);
       } else {
-        if (s & bit) movers[equal_w[i] + __popc(s & ~below_keep(i) & (bit - 1))] = j;
-        else w_out[j] = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (j + k >= s1) break;
+          if (j + k < p.keep) {
+            if (!same_w) w_out[j + k] = w[u][k];
+            if (!(same_pos && j + k < known)) pos_out[j + k] = pos[u][k];
+          } else if (!same_w || !(s >> (b + k) & 1)) {  // (in place a mover's weight is still to be read)
+            w_out[j + k] = 0.f;
+          }
+        }
+      }
+      const uint32_t lo = below_keep(i), hole = live(i) & lo & ~s, mover = s & ~lo;
+      for (uint32_t m = (hole | mover) >> b & 15u; m; m &= m - 1) {
+        const int k = b + __ffs(m) - 1;
+        const uint32_t before = (1u << k) - 1;
+        if (hole >> k & 1) holes[hole0[i] + __popc(hole & before)] = j - b + k;
+        else movers[equal_w[i] + __popc(mover & before)] = j - b + k;
       }
     }
   }
@@ -512,6 +550,7 @@ extern "C" int ms_launch_evict(void *k_pool, void *v_pool, int64_t pool_blocks, 
   p.num_kv_heads = num_kv_heads;
   p.chunks = head_dim * (dtype == MS_DTYPE_F32 ? 4 : 2) / 16;
   p.half = max_ctx / 2 + 1;
+  p.vec = stride % 4 == 0 && ptr16(weight_in) && ptr16(weight_out) && ptr16(pos_out) && (!pos_in || ptr16(pos_in));
   p.lists = static_cast<int32_t *>(workspace);
   p.moves = p.lists + size_t(num_rows) * num_kv_heads * 2 * p.half;
   cudaError_t e = standalone_status_word(&p.status);
