@@ -205,18 +205,19 @@ def test_bad_rows_are_skipped_and_flagged():
                 assert torch.equal(bits(a[pages]), bits(b[pages]))
 
 
-def test_stream_and_graph_replay():
-    ctx = [400, 333]
+@pytest.mark.parametrize("n,keep", [(400, 200), (4000, 1500)])  # one launch, two launches
+def test_stream_and_graph_replay(n, keep):
+    ctx = [n, n - 67]
     s = state(ctx, 2, 64, torch.bfloat16, 7)
-    want = expect(s, 200, 4, 50, ctx, [0, 0], torch.full_like(s["w"], 9.0), torch.full_like(s["pos"], -9))
-    dev = {n: s[n].to(DEV) for n in ("w", "pos", "k", "v", "tables", "rt")}
+    want = expect(s, keep, 4, 50, ctx, [0, 0], torch.full_like(s["w"], 9.0), torch.full_like(s["pos"], -9))
+    dev = {x: s[x].to(DEV) for x in ("w", "pos", "k", "v", "tables", "rt")}
     c = torch.tensor(ctx, dtype=torch.int32, device=DEV)
     lib = E.lib()
-    need = lib.ms_evict_workspace_bytes(2, 2, 400)
+    need = lib.ms_evict_workspace_bytes(2, 2, n)
 
     def call(stream, o):
         assert lib.ms_launch_evict(ptr(o["k"]), ptr(o["v"]), s["k"].shape[0], ptr(dev["tables"]), s["tables"].shape[0],
-                                   s["tables"].shape[1], ptr(dev["rt"]), ptr(c), ptr(c), None, 2, 400, 200, 4, 50,
+                                   s["tables"].shape[1], ptr(dev["rt"]), ptr(c), ptr(c), None, 2, n, keep, 4, 50,
                                    ptr(dev["w"]), ptr(o["w"]), None, ptr(o["pos"]), s["w"].shape[-1], 2, 64, 16,
                                    ptr(o["ws"]), need, 1, stream) == 0
 
@@ -224,12 +225,27 @@ def test_stream_and_graph_replay():
         return {"k": s["k"].to(DEV), "v": s["v"].to(DEV), "w": torch.full_like(dev["w"], 9.0),
                 "pos": torch.full_like(dev["pos"], -9), "ws": torch.empty(need, dtype=torch.uint8, device=DEV)}
 
+    def check_all(o):
+        for x, exp in zip(("k", "v", "w", "pos"), want):
+            assert torch.equal(bits(o[x]), bits(exp)), x
+
     side = [torch.cuda.Stream() for _ in range(2)]
     got = [buffers() for _ in side]
     torch.cuda.synchronize()
     for st, o in zip(side, got):
         call(st.cuda_stream, o)
     torch.cuda.synchronize()
+    for o in got:
+        check_all(o)
+    # one after the other in a stream, through the same workspace
+    first, second = buffers(), buffers()
+    second["ws"] = first["ws"]
+    torch.cuda.synchronize()
+    for o in (first, second):
+        call(None, o)
+    torch.cuda.synchronize()
+    check_all(first)
+    check_all(second)
     o = buffers()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
@@ -237,9 +253,7 @@ def test_stream_and_graph_replay():
     graph.replay()
     graph.replay()  # the same weights again: the same moves of the same values
     torch.cuda.synchronize()
-    for o in got + [o]:
-        for n, exp in zip(("k", "v", "w", "pos"), want):
-            assert torch.equal(bits(o[n]), bits(exp)), n
+    check_all(o)
     assert E.kernel_status(0) == 0
 
 
