@@ -663,9 +663,11 @@ cudaError_t launch_window_attention(const WindowArgs &a, cudaStream_t stream) {
   if (!common_ok(a) || !a.row_ctx || a.tiles || a.max_ctx > int64_t(a.max_blocks_per_seq) * attn::kBS ||
       (!a.row_table && a.table_rows < a.num_rows))
     return cudaErrorInvalidValue;
-  if (a.weight_sum && (a.row_index || a.weight_stride < a.max_ctx || !ptr16(a.workspace) ||
-                       a.workspace_bytes < attention_weights_workspace_bytes(a.num_rows, a.num_heads, a.max_ctx)))
-    return cudaErrorInvalidValue;
+  if (a.weight_sum) {
+    const int64_t need = attention_weights_workspace_bytes(a.num_rows, a.num_heads, a.max_ctx);
+    if (a.row_index || a.weight_stride < a.max_ctx || (need > 0 && !ptr16(a.workspace)) || a.workspace_bytes < need)
+      return cudaErrorInvalidValue;
+  }
   return launch_checked(a, stream);
 }
 

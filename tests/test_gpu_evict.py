@@ -98,9 +98,10 @@ def run(s, keep, sinks, recent, nxt, known, dt, in_place):
 @pytest.mark.parametrize("in_place", [False, True])
 @pytest.mark.parametrize("keep,sinks,recent", [(1, 0, 0), (1, 1, 0), (16, 0, 16), (33, 4, 5), (100, 0, 0), (100, 100, 0),
                                                (129, 4, 64), (700, 4, 100), (5000, 1, 1)])
-def test_first_eviction(keep, sinks, recent, in_place):
+@pytest.mark.parametrize("extra", [3, 5])  # the stride: a multiple of 4, and not
+def test_first_eviction(keep, sinks, recent, in_place, extra):
     ctx = [0, 1, 2, 16, 17, 34, 101, 130, 700, 1025]
-    s = state(ctx, 3, 64, torch.bfloat16, keep)
+    s = state(ctx, 3, 64, torch.bfloat16, keep, extra=extra)
     run(s, keep, sinks, recent, ctx, None, torch.bfloat16, in_place)
 
 
@@ -112,11 +113,12 @@ def test_types(name, d):
 
 
 @pytest.mark.parametrize("in_place", [False, True])
-def test_later_eviction_goes_by_positions(in_place):
+@pytest.mark.parametrize("extra", [4, 5])
+def test_later_eviction_goes_by_positions(in_place, extra):
     """Slots below row_known hold their own positions, in any order."""
     ctx, known = [300, 260, 200, 77], [256, 256, 0, 77]
     nxt = [900, 260 + 44, 200, 500]
-    s = state(ctx, 2, 64, torch.bfloat16, 5)
+    s = state(ctx, 2, 64, torch.bfloat16, 5, extra=extra)
     g = torch.Generator().manual_seed(1)
     for r, (c, kn, nx) in enumerate(zip(ctx, known, nxt)):
         for h in range(2):
@@ -151,6 +153,26 @@ def test_ties_and_special_weights(kind):
 def test_long(ctx, keep):
     s = state(ctx, 2, 64, torch.float16, keep)
     run(s, keep, 4, min(200, keep // 2), ctx, None, torch.float16, True)
+
+
+def test_pages_whose_elements_pass_32_bits():
+    hkv, d, dt, n, keep = 8, 128, torch.bfloat16, 100, 60
+    pool = (2 ** 31 // (hkv * 16 * d)) + 40
+    k, v = (torch.zeros(pool, hkv, 16, d, dtype=dt, device=DEV) for _ in range(2))
+    assert k.numel() > 2 ** 31
+    g = torch.Generator().manual_seed(8)
+    pages = torch.tensor([pool - 1, 3, pool - 9, pool // 2, pool - 2, 0, pool - 30])
+    s = {"tables": pages[None].to(torch.int32), "rt": torch.zeros(1, dtype=torch.int32), "ctx": [n],
+         "w": torch.rand(1, hkv, n, generator=g), "pos": torch.zeros(1, hkv, n, dtype=torch.int32)}
+    small_k, small_v = (torch.randn(7, hkv, 16, d, generator=g).to(dt) for _ in range(2))
+    k[pages.to(DEV)], v[pages.to(DEV)] = small_k.to(DEV), small_v.to(DEV)
+    w, pos = s["w"].to(DEV), s["pos"].to(DEV)
+    sync_ok(launch(s, keep, 2, 5, [n], None, w, w, pos, pos, k, v, dt))
+    assert E.kernel_status(0) == 0
+    local = dict(s, k=small_k, v=small_v, tables=torch.arange(7, dtype=torch.int32)[None])
+    want = expect(local, keep, 2, 5, [n], [0], s["w"], s["pos"])
+    for got, exp in ((k[pages.to(DEV)], want[0]), (v[pages.to(DEV)], want[1]), (w, want[2]), (pos, want[3])):
+        assert torch.equal(bits(got), bits(exp))
 
 
 def test_many_rows():

@@ -246,13 +246,14 @@ def run_weights(q, k, v, tables, rt, ctx, out, w, max_ctx=None, ws=None, stream=
 
 @pytest.mark.parametrize("name", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("group,hkv,d", [(1, 2, 64), (2, 2, 128), (4, 1, 64), (7, 2, 128), (8, 1, 128)])
-def test_weights_accumulate(name, group, hkv, d):
+@pytest.mark.parametrize("odd", [3, 2])  # the stride: a multiple of 4, and not
+def test_weights_accumulate(name, group, hkv, d, odd):
     dt = DTYPES[name]
     ctx = LENS + [1301]
     k, v, tables, rt = cache(ctx, [max(0, c - 1) for c in ctx], 0, 0, hkv, d, dt, 3)
     q = (2 * torch.randn(len(ctx), hkv * group, d, generator=torch.Generator().manual_seed(9))).to(dt)
     out = torch.full(q.shape, math.nan, dtype=dt, device=DEV)
-    stride = max(ctx) + 3
+    stride = max(ctx) + odd
     w0 = torch.rand(len(ctx), hkv, stride, generator=torch.Generator().manual_seed(2))
     wd = w0.to(DEV)
     dev = [x.to(DEV) for x in (q, k, v, tables, rt)]
@@ -293,6 +294,49 @@ def test_weights_equal_calls_give_equal_bits():
         if first is None:
             first = (out, w)
         assert torch.equal(out, first[0]) and torch.equal(w, first[1])
+
+
+def test_weights_with_nothing_cached():
+    q = torch.randn(2, 4, 64, device=DEV).bfloat16()
+    pool = torch.zeros(1, 2, 16, 64, dtype=torch.bfloat16, device=DEV)
+    out, w = torch.full_like(q, 5.0), torch.full((2, 2, 8), 3.0, device=DEV)
+    tables, zero = torch.zeros(2, 1, dtype=torch.int32, device=DEV), torch.zeros(2, dtype=torch.int32, device=DEV)
+    rc = E.lib().ms_launch_attention_weights(ptr(q), ptr(pool), ptr(pool), 1, ptr(tables), 2, 1, None, ptr(zero), 2, 0, ptr(out),
+                                             ptr(w), 8, 4, 2, 64, 16, 0.125, None, 0, 1, None)
+    sync_ok(rc)
+    assert E.kernel_status(0) == 0 and (out == 0).all() and (w == 3.0).all()
+
+
+def test_pages_whose_elements_pass_32_bits():
+    """A pool of 2^31 elements and more: its last pages, in every operator that reads them."""
+    hkv, d, dt, n = 8, 128, torch.bfloat16, 100
+    pool = (2 ** 31 // (hkv * 16 * d)) + 40
+    k, v = (torch.zeros(pool, hkv, 16, d, dtype=dt, device=DEV) for _ in range(2))
+    assert k.numel() > 2 ** 31
+    g = torch.Generator().manual_seed(8)
+    pages = torch.tensor([pool - 1, 3, pool - 9, pool // 2, pool - 2, 0, pool - 30], dtype=torch.int32)
+    small_k, small_v = (torch.randn(7, hkv, 16, d, generator=g).to(dt) for _ in range(2))
+    k[pages.long().to(DEV)], v[pages.long().to(DEV)] = small_k.to(DEV), small_v.to(DEV)
+    tables, rt = pages[None].clone(), torch.zeros(1, dtype=torch.int32)
+    q = (2 * torch.randn(1, 16, d, generator=g)).to(dt)
+    local = torch.arange(7, dtype=torch.int32)[None]
+    qd, td, rd = q.to(DEV), tables.to(DEV), rt.to(DEV)
+    for window, sinks in ((0, 0), (40, 3)):
+        out = torch.full(q.shape, math.nan, dtype=dt, device=DEV)
+        sync_ok(run_rows(qd, k, v, td, rd, [n], window, sinks, out))
+        want, _, absv, smax = ref.window_rows(q, small_k, small_v, local, rt, [n], window, sinks, ref.scale_of(d))
+        check(out, want, absv, smax, n, dt)
+        tl = torch.tensor([[0, 1, n - 1, 0]], dtype=torch.int32, device=DEV)
+        out = torch.full(q.shape, math.nan, dtype=dt, device=DEV)
+        sync_ok(E.lib().ms_launch_window_prefill(ptr(qd), ptr(k), ptr(v), pool, ptr(td), 1, 7, ptr(tl), 1, window, sinks,
+                                                 ptr(out), 16, hkv, d, 16, ref.scale_of(d), dt_code(q), None))
+        check(out, want, absv, smax, n, dt, exp_err=8e-5)
+    out, w = torch.full(q.shape, math.nan, dtype=dt, device=DEV), torch.zeros(1, hkv, n, device=DEV)
+    sync_ok(run_weights(qd, k, v, td, rd, [n], out, w))
+    want, add, absv, smax = ref.window_rows(q, small_k, small_v, local, rt, [n], 0, 0, ref.scale_of(d))
+    check(out, want, absv, smax, n, dt)
+    assert float((w[0].cpu().double() - add[0]).abs().max()) < 1e-5
+    assert E.kernel_status(0) == 0
 
 
 # ---- values in device memory that are out of range ----------------------------------
