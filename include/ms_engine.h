@@ -486,7 +486,7 @@ int ms_launch_attention_weights(const void *q, const void *k_pool, const void *v
  * slots) and may free the pages behind it.
  *  - Slot j holds position pos_in[table row][kv head][j] for j < row_known[t]
  *    (slots an earlier eviction placed) and row_next[t] - n + j from there on
- *    (tokens appended since), row_next[t] = tokens the sequence has seen.
+ *    (tokens appended since), row_next[t] >= n: tokens the sequence has seen.
  *    row_known may be NULL: 0, pos_in is then not read and may be NULL.
  *  - Kept are the slots with position < sinks or >= row_next[t] - recent, and
  *    of the others those with the largest weight_in[table row][kv head][j],
