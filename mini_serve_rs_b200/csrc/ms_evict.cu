@@ -25,7 +25,7 @@
 // once on as many warps, because a row in a large pool costs a long latency
 // (address translation included) and few bytes: with the moves left to the CTA
 // that selected them, 8 at a time per warp, the longest sequences of a ragged
-// batch finished long after the others (64 sequences: 68 us against 33).
+// batch finished long after the others (64 sequences: 68 us against 44).
 // Latency-bound for one sequence (a chain of loads and barriers), bound by the
 // moves' HBM traffic for many.
 #include <algorithm>
