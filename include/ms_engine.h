@@ -435,7 +435,8 @@ int ms_prefill_tiles(const int32_t *seq_row0, const int32_t *seq_ntok, const int
  *  - Host arguments out of range return cudaErrorInvalidValue before anything
  *    is launched.  What lies in device memory is checked by the kernels: a row
  *    (tile) whose context, positions or table row are out of range is skipped,
- *    its outputs stay as they were; a page id outside [0, pool_blocks) is
+ *    its outputs stay as they were (an empty one, row_ctx or rows 0 as in a
+ *    padded batch, may name any table row); a page id outside [0, pool_blocks) is
  *    never dereferenced, and the row that names it gets an unspecified result.
  *    Both set bit 2 of the status word that ms_kernel_status returns.
  *  - Table entries of pages that hold no key any row sees are not read, so the

@@ -219,12 +219,13 @@ __global__ void __launch_bounds__(NT, 1024 / NT) evict_kernel(EvictParams p, int
   __shared__ Shared sh;
   const int row = blockIdx.x / C, part = blockIdx.x % C, h = blockIdx.y;
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
-  const int n = p.row_ctx[row], next = p.row_next[row], trow = p.row_table ? p.row_table[row] : row;
+  const int n = p.row_ctx[row], next = p.row_next[row];
+  const int trow = n == 0 ? 0 : p.row_table ? p.row_table[row] : row;  // an empty row names none
   const int known = p.row_known ? p.row_known[row] : 0;
   for (int i = t; i < kDigits * kBins / 4; i += NT)
     reinterpret_cast<uint4 *>(sh.hist)[i] = make_uint4(0, 0, 0, 0);
-  bool ok = n >= 0 && n <= p.max_ctx && trow >= 0 && trow < p.table_rows && known >= 0 && next >= n;
-  if (table_row_repeated(p.row_table, row, trow)) ok = false;  // (with a barrier)
+  bool ok = n == 0 || (n > 0 && n <= p.max_ctx && trow >= 0 && trow < p.table_rows && known >= 0 && next >= n);
+  if (table_row_repeated(p.row_table, p.row_ctx, row, trow) && n != 0) ok = false;  // (with a barrier)
   const size_t pair = size_t(row) * p.num_kv_heads + h;
   if (!ok) {  // the whole cluster leaves
     if (t == 0) {

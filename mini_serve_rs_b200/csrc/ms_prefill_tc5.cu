@@ -321,12 +321,12 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
   }
   if constexpr (WIN) {
-    if (row0 < 0 || nrows < 0 || nrows > kHalves * TPH || pos0 < 0 || trow < 0 || trow >= p.table_rows ||
-        pos0 > p.max_blocks_per_seq * kBS - nrows) {
+    if (nrows != 0 && (row0 < 0 || nrows < 0 || nrows > kHalves * TPH || pos0 < 0 || trow < 0 ||
+                       trow >= p.table_rows || pos0 > p.max_blocks_per_seq * kBS - nrows)) {
       if (t == 0) atomicOr(p.status, kStatusBadIndex);
-      row0 = nrows = pos0 = trow = 0;  // an empty tile: nothing is loaded or stored
+      nrows = 0;
     }
-    if (nrows == 0) pos0 = 0;
+    if (nrows == 0) row0 = pos0 = trow = 0;  // an empty tile: nothing is loaded or stored
   }
   const int32_t *table = p.block_tables + size_t(trow) * p.max_blocks_per_seq;
   int kv_len = pos0 + nrows;

@@ -336,9 +336,10 @@ __global__ void __launch_bounds__(Page::WARPS * 32)
   const int row = p.row_index ? p.row_index[ri] : ri;
   const int kvh = blockIdx.y, G = p.group;
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
-  const int ctx = p.row_ctx[row], trow = p.row_table ? p.row_table[row] : row;
+  const int ctx = p.row_ctx[row];
+  const int trow = ctx == 0 ? 0 : p.row_table ? p.row_table[row] : row;  // an empty row names none
   bool ok = ctx >= 0 && ctx <= p.max_ctx && trow >= 0 && trow < p.table_rows;
-  if (WEIGHTS && table_row_repeated(p.row_table, row, trow)) ok = false;
+  if (WEIGHTS && table_row_repeated(p.row_table, p.row_ctx, row, trow) && ctx != 0) ok = false;
   if (!ok) {  // the whole cluster leaves
     if (t == 0) atomicOr(p.status, kStatusBadIndex);
     return;

@@ -34,11 +34,13 @@ struct VisiblePages {
 };
 
 // Rows of one call that name the same table row: the first one counts.  Every
-// thread of the CTA calls this; true when an earlier row names `table_row`.
-__device__ __forceinline__ bool table_row_repeated(const int32_t *row_table, int row, int table_row) {
+// thread of the CTA calls this; true when an earlier row that holds anything
+// (a padded batch's rows do not) names `table_row`.
+__device__ __forceinline__ bool table_row_repeated(const int32_t *row_table, const int32_t *row_ctx, int row,
+                                                   int table_row) {
   int found = 0;
   if (row_table)
-    for (int i = threadIdx.x; i < row; i += blockDim.x) found |= row_table[i] == table_row;
+    for (int i = threadIdx.x; i < row; i += blockDim.x) found |= row_table[i] == table_row && row_ctx[i] > 0;
   return __syncthreads_or(found) != 0;
 }
 

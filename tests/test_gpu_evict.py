@@ -181,6 +181,20 @@ def test_many_rows():
     run(s, 128, 4, 32, ctx, None, torch.bfloat16, True)
 
 
+def test_padded_batch():
+    """Empty rows may name any table row, a used one or none, before it or after."""
+    ctx = [100, 120]
+    s = state(ctx, 2, 64, torch.bfloat16, 6)
+    want = expect(s, 64, 4, 16, ctx, [0, 0], s["w"], s["pos"])
+    w, pos, k, v = (s[n].to(DEV) for n in ("w", "pos", "k", "v"))
+    padded = dict(s, ctx=[0, 100, 0, 120, 0])
+    rt = torch.tensor([s["rt"][0], s["rt"][0], -7, s["rt"][1], s["rt"][1]], dtype=torch.int32)
+    sync_ok(launch(padded, 64, 4, 16, [0, 100, -3, 120, 9], [0, 0, -1, 0, 0], w, w, pos, pos, k, v, torch.bfloat16, rt=rt))
+    assert E.kernel_status(0) == 0
+    for got, exp in ((k, want[0]), (v, want[1]), (w, want[2]), (pos, want[3])):
+        assert torch.equal(bits(got), bits(exp))
+
+
 def test_bad_rows_are_skipped_and_flagged():
     ctx = [100, 120, 140]
     s = state(ctx, 2, 64, torch.bfloat16, 6)

@@ -412,6 +412,63 @@ def test_weights_of_a_repeated_table_row_are_flagged():
     assert (w2[rt[2].long()] == 0).all()
 
 
+def test_padded_batches():
+    """Empty rows and tiles may name any table row, a used one or none."""
+    hkv, d, dt = 2, 64, torch.bfloat16
+    ctx = [40, 50]
+    k, v, tables, rt = cache(ctx, [0, 0], 0, 0, hkv, d, dt, 11)
+    q = torch.randn(5, 4, d).to(dt)
+    dev = [x.to(DEV) for x in (q, k, v, tables)]
+    real = [1, 3]
+    plain = [dev[0][real].contiguous()] + dev[1:]
+    out, w = torch.full((2, 4, d), 5.0, dtype=dt, device=DEV), torch.zeros(2, hkv, 64, device=DEV)
+    sync_ok(run_weights(*plain, rt.to(DEV), ctx, out, w))
+    padded_rt = torch.tensor([rt[0], rt[0], -7, rt[1], rt[1]], dtype=torch.int32, device=DEV)
+    out2, w2 = torch.full(q.shape, 5.0, dtype=dt, device=DEV), torch.zeros(2, hkv, 64, device=DEV)
+    sync_ok(run_weights(*dev, padded_rt, [0, 40, 0, 50, 0], out2, w2))
+    assert E.kernel_status(0) == 0
+    assert torch.equal(out2[real], out) and torch.equal(w2, w) and (out2[[0, 2, 4]] == 0).all()
+    out3 = torch.full(q.shape, 5.0, dtype=dt, device=DEV)
+    sync_ok(run_rows(*dev, padded_rt, [0, 40, 0, 50, 0], 0, 0, out3))
+    assert E.kernel_status(0) == 0 and torch.equal(out3[real], out) and (out3[[0, 2, 4]] == 0).all()
+    chunk = torch.full((2, 4, d), 5.0, dtype=dt, device=DEV)
+    tl = torch.tensor([[0, 1, 39, rt[0]], [-9, 0, -1, 77], [1, 1, 49, rt[1]], [0, 0, 1 << 30, -1]], dtype=torch.int32, device=DEV)
+    sync_ok(E.lib().ms_launch_window_prefill(ptr(plain[0]), ptr(dev[1]), ptr(dev[2]), k.shape[0], ptr(dev[3]), 2,
+                                             tables.shape[1], ptr(tl), 4, 0, 0, ptr(chunk), 4, hkv, d, 16, ref.scale_of(d),
+                                             dt_code(q), None))
+    assert E.kernel_status(0) == 0
+    want, _, absv, smax = want_rows(q[real], k, v, tables, rt, ctx, 0, 0)
+    check(chunk, want, absv, smax, 50, dt, exp_err=8e-5)
+
+
+def test_no_row_table_and_very_many_rows():
+    hkv, d, dt = 1, 64, torch.bfloat16
+    k, v, tables, _ = cache([40, 50, 60], [0, 0, 0], 0, 0, hkv, d, dt, 13)
+    rt = torch.arange(3, dtype=torch.int32)
+    order = torch.argsort(cache([40, 50, 60], [0, 0, 0], 0, 0, hkv, d, dt, 13)[3])
+    ctx = [[40, 50, 60][int(i)] for i in order]  # of table rows 0, 1, 2
+    q = torch.randn(3, 4, d).to(dt)
+    dev = [x.to(DEV) for x in (q, k, v, tables, rt)]
+    named, unnamed = (torch.full(q.shape, 5.0, dtype=dt, device=DEV) for _ in range(2))
+    sync_ok(run_rows(*dev, ctx, 30, 2, named))
+    cd = torch.tensor(ctx, dtype=torch.int32, device=DEV)
+    call = (ptr(dev[1]), ptr(dev[2]), k.shape[0], ptr(dev[3]), 3, tables.shape[1])
+    rc = E.lib().ms_launch_window_attention(ptr(dev[0]), *call, None, ptr(cd), 3, 60, 30, 2, ptr(unnamed), 4, hkv, d, 16,
+                                            ref.scale_of(d), 1, None)
+    sync_ok(rc)
+    assert E.kernel_status(0) == 0 and torch.equal(named, unnamed)
+    rows = 70001  # more than a grid's y or z holds
+    many_q = dev[0][:1].expand(rows, -1, -1).contiguous()
+    out = torch.full(many_q.shape, 5.0, dtype=dt, device=DEV)
+    zeros, many_ctx = torch.zeros(rows, dtype=torch.int32, device=DEV), torch.full((rows,), ctx[0], dtype=torch.int32, device=DEV)
+    sync_ok(E.lib().ms_launch_window_attention(ptr(many_q), ptr(dev[1]), ptr(dev[2]), k.shape[0], ptr(dev[3]), 3,
+                                               tables.shape[1], ptr(zeros), ptr(many_ctx), rows, 60, 30, 2, ptr(out), 4, hkv, d,
+                                               16, ref.scale_of(d), 1, None))
+    assert E.kernel_status(0) == 0 and (out == out[:1]).all()
+    want, _, absv, smax = want_rows(q[:1], k, v, tables, rt, ctx[:1], 30, 2)
+    check(out[:1], want, absv, smax, 60, dt)
+
+
 # ---- streams and graphs ---------------------------------------------------------------
 
 def test_streams_and_graph_replay():
