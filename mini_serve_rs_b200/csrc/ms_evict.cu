@@ -451,8 +451,8 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(EvictParams p)
 }
 
 // CTAs per (sequence, kv head): enough to fill the machine (two on each of the 148 SMs), with
-// at least 4096 slots each (a cluster barrier costs as much as 4096 slots' share of a digit),
-// and as many as the rank keys need.
+// at least 4096 slots each (one sequence of 2176 slots: one CTA a head 10.4 us, two 15.5: each
+// digit then costs two cluster barriers), and as many as the rank keys need.
 int evict_cluster(int rows, int hkv, int max_ctx) {
   int c = 1;
   while (c < kMaxCluster &&
@@ -560,10 +560,12 @@ extern "C" int ms_launch_evict(void *k_pool, void *v_pool, int64_t pool_blocks, 
   if ((long long)num_rows * C > 0x7fffffffLL) return int(cudaErrorInvalidValue);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int most = std::max(0, std::min(keep, max_ctx - keep));  // moves of one head
-  // One launch where every warp of the cluster has at most one round of moves: a second launch
-  // costs the host 5 us and the GPU 1 us.
+  // One launch where every warp of the cluster has at most one round of moves (one sequence, 128
+  // moves a head: 13 us a call, 16 with a second launch, which costs the host more than the GPU;
+  // 64 sequences with up to 512 moves: 124 us of GPU time in one launch, 43 in two).
   if ((long long)most <= C * (512LL / 32) * 4 * (32 / p.chunks)) return int(launch_evict<512, true>(p, num_rows, C, st));
-  // small CTAs, four to an SM, where there are enough of them to fill it that way
+  // small CTAs, four to an SM, where there are enough of them to fill it that way (64 sequences:
+  // 43 us, CTAs of 512 46 us)
   const bool many = (long long)num_rows * num_kv_heads * C >= 2 * 148;
   e = many ? launch_evict<256, false>(p, num_rows, C, st) : launch_evict<512, false>(p, num_rows, C, st);
   if (e == cudaSuccess) e = launch_moves(p, num_rows, most, st);
