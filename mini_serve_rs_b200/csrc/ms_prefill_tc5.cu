@@ -324,9 +324,9 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
     if (nrows != 0 && (row0 < 0 || nrows < 0 || nrows > kHalves * TPH || pos0 < 0 || trow < 0 ||
                        trow >= p.table_rows || pos0 > p.max_blocks_per_seq * kBS - nrows)) {
       if (t == 0) atomicOr(p.status, kStatusBadIndex);
-      nrows = 0;
+      row0 = nrows = pos0 = trow = 0;
     }
-    if (nrows == 0) row0 = pos0 = trow = 0;  // an empty tile: nothing is loaded or stored
+    if (nrows == 0) pos0 = 0;  // an empty tile has no pages: nothing is loaded or stored
   }
   const int32_t *table = p.block_tables + size_t(trow) * p.max_blocks_per_seq;
   int kv_len = pos0 + nrows;
