@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
   __shared__ int mma_landed_s, issued_s;
 
   const int kvh = blockIdx.x, tile = blockIdx.y;  // kv heads vary fastest: a tile's heads start together
-  const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+  const int t = threadIdx.x, warp = __shfl_sync(kFull, t >> 5, 0), lane = t & 31;  // warp: uniform, and known to be
   int row0 = p.tiles[tile * 4 + 0], nrows = p.tiles[tile * 4 + 1];
   int pos0 = p.tiles[tile * 4 + 2], trow = p.tiles[tile * 4 + 3];
   // warp 8 sets up while the others fetch their first operands
