@@ -448,7 +448,10 @@ int ms_prefill_tiles(const int32_t *seq_row0, const int32_t *seq_ntok, const int
  * row_ctx[t] - 1, attends to the keys j <= p with p - j < window or j < sinks
  * (window = 0: to all j <= p); a row with row_ctx[t] = 0 gets zeros.
  * row_table may be NULL (row t uses table row t; table_rows >= num_rows).
- * Softmax in f32, one rounding of the result.  One launch, no workspace. */
+ * Scores, maxima and sums in f32, one rounding of the result.  With 16-bit K/V
+ * the weights are rounded to that type for their product with V: half a step
+ * of each, in f16 down to 2^-29 of the row's heaviest, 2^-40 of the heaviest
+ * below that.  One launch, no workspace. */
 int ms_launch_window_attention(const void *q, const void *k_pool, const void *v_pool, int64_t pool_blocks,
                                const int32_t *block_tables, int32_t table_rows, int32_t max_blocks_per_seq,
                                const int32_t *row_table, const int32_t *row_ctx, int32_t num_rows,

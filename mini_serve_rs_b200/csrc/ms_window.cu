@@ -34,6 +34,7 @@
 // them back once the cluster has exchanged the maxima and sums.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "ms_window.cuh"
 
@@ -64,6 +65,10 @@ template <typename T_, int D_> struct PageTc {
   using T = T_;
   static constexpr int D = D_, WARPS = 4, NSTAGE = D == 128 ? 2 : 3;
   static constexpr int NDH = D / 64, TILE_BYTES = NDH * kHalfBytes, KSTEPS = D / 16, NTD = D / 8;
+  // P <= 1 is stored as 2^15 P in f16, whose numbers are of full precision from 2^-14 to 2^16 only
+  // (bf16 has f32's range): without it keys 2^-25 as heavy as the heaviest vanished from O but not
+  // from the sum.  store() takes the factor out again.
+  static constexpr float kScaleP = std::is_same<T, __half>::value ? 32768.f : 1.f;
   uint32_t qa[KSTEPS][2];
   float o[NTD][4];
   float m_run = -INFINITY, l_run = 0.f;
@@ -150,8 +155,9 @@ template <typename T_, int D_> struct PageTc {
       o[nd][1] *= alpha;
     }
     // P is rounded to the K/V type for the tensor cores (the sum above is not): half a step
-    // relative per weight, which the result's own rounding matches
-    const uint32_t pa[4] = {pack2<T>(pj[0], pj[1]), 0u, pack2<T>(pj[2], pj[3]), 0u};
+    // relative per weight, which the result's own rounding matches; in f16 below 2^-29 of the
+    // heaviest key half of 2^-39 of that key's weight
+    const uint32_t pa[4] = {pack2<T>(pj[0] * kScaleP, pj[1] * kScaleP), 0u, pack2<T>(pj[2] * kScaleP, pj[3] * kScaleP), 0u};
 #pragma unroll
     for (int ndp = 0; ndp < NTD / 2; ++ndp) {
       uint32_t b[4];
@@ -169,7 +175,8 @@ template <typename T_, int D_> struct PageTc {
     if (gid >= group) return;
 #pragma unroll
     for (int nd = 0; nd < NTD; ++nd)
-      *reinterpret_cast<float2 *>(mo + gid * D + nd * 8 + 2 * tig) = make_float2(o[nd][0], o[nd][1]);
+      *reinterpret_cast<float2 *>(mo + gid * D + nd * 8 + 2 * tig) =
+          make_float2(o[nd][0] * (1.f / kScaleP), o[nd][1] * (1.f / kScaleP));
     if (tig == 0) {
       mm[gid] = m_run;
       ml[gid] = l_run;

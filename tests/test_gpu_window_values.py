@@ -1,0 +1,94 @@
+"""Values that test the arithmetic of ms_launch_window_attention,
+ms_launch_window_prefill and ms_launch_attention_weights: weights far below the
+heaviest one, NaN and infinity where a row sees them, large numbers where it
+does not."""
+import math
+
+import pytest
+import torch
+
+from mini_serve_rs_b200 import engine as E
+from oracle import bounded_cache_ref as ref
+from tests.gpu_util import dt_code, need_gpu, ptr, sync_ok
+from tests.test_gpu_window import DEV, DTYPES, run_rows, run_weights, tiles_of
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _gpu():
+    need_gpu()
+    E.kernel_status(0)
+
+
+def one_sequence(k, v):
+    """Keys and values [n, Hkv, D] as pools, block table and row table of one sequence."""
+    n, hkv, d = k.shape
+    blocks = -(-n // 16)
+    pools = []
+    for x in (k, v):
+        p = torch.zeros(blocks * 16, hkv, d, dtype=x.dtype)
+        p[:n] = x
+        pools.append(p.reshape(blocks, 16, hkv, d).transpose(1, 2).contiguous())
+    perm = torch.randperm(blocks, generator=torch.Generator().manual_seed(n))
+    tables = torch.empty(1, blocks, dtype=torch.int32)
+    tables[0] = perm.to(torch.int32)
+    for i, p in enumerate(pools):
+        pools[i] = torch.empty_like(p)
+        pools[i][perm] = p
+    return pools[0], pools[1], tables, torch.zeros(1, dtype=torch.int32)
+
+
+def run_chunk(q, k, v, tables, tl, window, sinks, out):
+    return E.lib().ms_launch_window_prefill(
+        ptr(q.to(DEV)), ptr(k.to(DEV)), ptr(v.to(DEV)), k.shape[0], ptr(tables.to(DEV)), tables.shape[0], tables.shape[1],
+        ptr(tl.to(DEV)), len(tl), window, sinks, ptr(out), q.shape[1], k.shape[1], q.shape[2], 16,
+        ref.scale_of(q.shape[2]), dt_code(q), None)
+
+
+def tails(dt, d, far, heavy, n=16384):
+    """One key that takes nearly all the weight and whose value is 0, and n keys 2^far below it
+    whose values are 16 to 32: what a row returns is the light keys' share alone."""
+    g = torch.Generator().manual_seed(int(far * 10))
+    k, v = torch.zeros(n + 1, 1, d), 16 + 16 * torch.rand(n + 1, 1, d, generator=g)
+    k[:, 0, 0] = -far * math.log(2.0) * math.sqrt(d) / 8
+    k[heavy], v[heavy] = 0.0, 0.0
+    q = torch.zeros(1, 2, d)
+    q[..., 0] = 8.0
+    return q.to(dt), k.to(dt), v.to(dt)
+
+
+def tail_tolerance(dt, want, absv, n, exp_err):
+    """oracle.bounded_cache_ref.bound without its constant term: each weight keeps the relative
+    precision of its type however light it is, the result is rounded once (half a subnormal step
+    at least).  Sums of n f32 terms of one sign: 2^-23 each.  The scores are one exact product each."""
+    half = torch.finfo(dt).eps / 2
+    rel = 2 * exp_err + (n + 64) * 2.0 ** -23 + 2 * 2.0 ** -23 * 64 + (half if dt != torch.float32 else 0.0)
+    step = torch.finfo(dt).smallest_normal * torch.finfo(dt).eps
+    return half * want.abs() * 1.001 + rel * absv + step / 2
+
+
+@pytest.mark.parametrize("name,d", [("f16", 128), ("f16", 64), ("bf16", 128), ("f32", 64)])
+@pytest.mark.parametrize("far", [8.0, 15.3, 20.7, 25.5, 28.0])
+@pytest.mark.parametrize("heavy", [0, 16384])
+def test_rows_keep_light_weights(name, d, far, heavy):
+    dt = DTYPES[name]
+    q, k, v = tails(dt, d, far, heavy)
+    n = k.shape[0]
+    kp, vp, tables, rt = one_sequence(k, v)
+    want, add, absv, _ = ref.window_rows(q, kp, vp, tables, rt, [n], 0, 0, ref.scale_of(d))
+    tol = tail_tolerance(dt, want, absv, n, 2.0 ** -20)
+    assert float((tol / want).max()) < 0.02  # far below what is measured
+    w = torch.zeros(1, 1, n + 3, device=DEV)
+    for op in ("window", "sinks and window", "weights"):
+        out = torch.full(q.shape, math.nan, dtype=dt, device=DEV)
+        if op == "weights":
+            sync_ok(run_weights(q.to(DEV), kp.to(DEV), vp.to(DEV), tables.to(DEV), rt.to(DEV), [n], out, w))
+        else:
+            sync_ok(run_rows(q, kp, vp, tables, rt, [n], 0 if op == "window" else n - 16, 0 if op == "window" else 16, out))
+        worst = float(((out.cpu().double() - want).abs() / tol).max())
+        print(f"{op}: worst error / bound {worst:.3f}")
+        assert worst <= 1.0, op
+    got = w[0, :, :n].cpu().double()
+    assert float(((got - add[0]).abs() / add[0]).max()) < 2 * 2.0 ** -20 + (n + 200) * 2.0 ** -23
+    assert E.kernel_status(0) == 0
