@@ -461,7 +461,9 @@ int ms_launch_window_attention(const void *q, const void *k_pool, const void *v_
 
 /* K3pw: K3p with the same window and sinks, bf16 / f16; tiles as for
  * ms_launch_paged_prefill (ms_prefill_tiles): the row at position p of a tile
- * attends to the keys j <= p with p - j < window or j < sinks. */
+ * attends to the keys j <= p with p - j < window or j < sinks.  Weights are
+ * rounded to the K/V type as in K3w (f16: whole down to 2^-25 of the row's
+ * heaviest), and some 2^x are good to 7.5e-5. */
 int ms_launch_window_prefill(const void *q, const void *k_pool, const void *v_pool, int64_t pool_blocks,
                              const int32_t *block_tables, int32_t table_rows, int32_t max_blocks_per_seq,
                              const int32_t *tiles, int32_t num_tiles, int32_t window, int32_t sinks, void *out,

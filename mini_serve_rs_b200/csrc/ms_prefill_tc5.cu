@@ -19,7 +19,7 @@
 //     run the online softmax in base 2 with the scale folded into one FMA
 //     before 2^x.  The running max moves only when the group's max exceeds it
 //     by more than 8 (then the warp rescales its O rows in TMEM), so
-//     P = 2^(s - m) stays <= 256.  P, rounded to the K/V type, is stored over
+//     P = 2^(s - m) stays <= 256 (windowed f16: Reference).  P, rounded to the K/V type, is stored over
 //     S(g)'s own TMEM columns (two 16-bit values per column) and the warp
 //     arrives on p_ready;
 //   * warp 8, one thread, MMAs in the order S_A(0) S_B(0) | PV_A(g) S_A(g+1)
@@ -71,7 +71,15 @@ namespace {
 
 constexpr int kRows = 128;     // query rows per CTA = TMEM lanes
 constexpr int kKeys = 128;     // keys per group (8 pages): the S MMA is M 128 x N 128
-constexpr float kRescale = 8.0f;  // move the running max only when it grows by more than 2^8
+// The row's reference moves only when the maximum passes it by more than kGrow, and then to kDrop
+// below the maximum, so P = 2^(s - reference) stays <= 2^kGrow.  bf16 has f32's range: 8 and 0.
+// f16 is of full precision from 2^-14 to 2^16 only: 15 and 11 keep keys down to 2^-25 of the
+// heaviest whole (8 and 0: to 2^-14; 16384 keys 2^24.5 below one of value 0 came out 5 % off in
+// the one of 8 shares that held it).  The causal build keeps 8 and 0 in both types.
+template <typename T, bool WIN> struct Reference {
+  static constexpr bool kF16 = WIN && std::is_same<T, __half>::value;
+  static constexpr float kGrow = kF16 ? 15.f : 8.f, kDrop = kF16 ? 11.f : 0.f;
+};
 constexpr int kExp2OnFma = 3;     // of every 8 score pairs, this many take 2^x on the FMA pipe (exp2_poly2)
 
 __device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t addr, uint32_t lbo_bytes, uint32_t sbo_bytes) {
@@ -214,7 +222,7 @@ __device__ __forceinline__ float max3f(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-// 2^x for two x <= 8 on the FMA and integer pipes instead of the transcendental unit
+// 2^x for two x <= 15 on the FMA and integer pipes instead of the transcendental unit
 // (Cody and Waite's argument split): j = rint(x) by adding and subtracting 1.5 * 2^23,
 // f = x - j in [-0.5, 0.5], 2^f by a cubic fitted here for relative error on [-0.5, 0.5]
 // (7.5e-5 at most in f32 Horner form), and j added to the exponent field.  x is clamped at
@@ -496,11 +504,12 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
       };
       const float mt = diag ? row_max(std::true_type{}) : row_max(std::false_type{});
       const float mts = mt * c;
-      const bool grow = mts > m_run + kRescale;  // m_run = -inf: any finite max
+      const bool grow = mts > m_run + Reference<T, WIN>::kGrow;  // m_run = -inf: any finite max
       float alpha = 1.f;
       if (grow) {
-        alpha = ex2_approx(m_run - mts);
-        m_run = mts;
+        const float m_new = mts - Reference<T, WIN>::kDrop;
+        alpha = ex2_approx(m_run - m_new);
+        m_run = m_new;
       }
       if (g > 0 && __any_sync(kFull, grow)) {
         // O is being accumulated by PV(g - 1): wait for it, then rescale this warp's rows

@@ -92,3 +92,55 @@ def test_rows_keep_light_weights(name, d, far, heavy):
     got = w[0, :, :n].cpu().double()
     assert float(((got - add[0]).abs() / add[0]).max()) < 2 * 2.0 ** -20 + (n + 200) * 2.0 ** -23
     assert E.kernel_status(0) == 0
+
+
+@pytest.mark.parametrize("name,d", [("f16", 128), ("f16", 64), ("bf16", 128)])
+@pytest.mark.parametrize("far", [8.0, 15.3, 20.7, 24.5])
+@pytest.mark.parametrize("heavy", [0, 16350])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (16300, 100)])
+def test_chunks_keep_light_weights(name, d, far, heavy, window, sinks):
+    """The tiles' reference may lie 2^4 below the maximum: weights from 2^-25 on are as precise as any."""
+    dt = DTYPES[name]
+    q, k, v = tails(dt, d, far, heavy)
+    n = k.shape[0]
+    kp, vp, tables, rt = one_sequence(k, v)
+    rows = 3
+    q = q.expand(rows, 2, d).contiguous()
+    tl = tiles_of([(n - rows, rows)], rt, 2)
+    out = torch.full(q.shape, math.nan, dtype=dt, device=DEV)
+    sync_ok(run_chunk(q, kp, vp, tables, tl, window, sinks, out))
+    assert E.kernel_status(0) == 0
+    want, _, absv, _ = ref.window_rows(q, kp, vp, tables, rt.expand(rows), [n - rows + 1 + i for i in range(rows)], window,
+                                       sinks, ref.scale_of(d))
+    tol = tail_tolerance(dt, want, absv, n, 8e-5)
+    worst = float(((out.cpu().double() - want).abs() / tol).max())
+    print(f"worst error / bound {worst:.3f}")
+    assert worst <= 1.0
+
+
+@pytest.mark.parametrize("name", ["f16", "bf16"])
+@pytest.mark.parametrize("step", [0.5, 3.9, 4.1, 7.9, 8.1])
+def test_chunks_whose_scores_climb(name, step):
+    """Each group of 128 keys is 2^step heavier than the one before it."""
+    dt, d, n = DTYPES[name], 64, 128 * 9 + 5
+    g = torch.Generator().manual_seed(2)
+    k, v = torch.zeros(n, 1, d), torch.randn(n, 1, d, generator=g)
+    k[:, 0, 0] = (torch.arange(n) // 128) * step * math.log(2.0) * math.sqrt(d) / 8
+    k[:, 0, 1] = 0.02 * torch.randn(n, generator=g)
+    q = torch.zeros(40, 2, d)
+    q[..., 0] = 8.0
+    q[..., 1] = torch.randn(40, 2, generator=g)
+    q, k, v = q.to(dt), k.to(dt), v.to(dt)
+    kp, vp, tables, rt = one_sequence(k, v)
+    for window in (0, 700):
+        tl = tiles_of([(n - 40, 40)], rt, 2)
+        out = torch.full(q.shape, math.nan, dtype=dt, device=DEV)
+        sync_ok(run_chunk(q, kp, vp, tables, tl, window, 0, out))
+        want, _, absv, _ = ref.window_rows(q, kp, vp, tables, rt.expand(40), [n - 39 + i for i in range(40)], window, 0,
+                                           ref.scale_of(d))
+        # scores up to 65 in two exact products: 2^-23 of that, twice
+        tol = tail_tolerance(dt, want, absv, n, 8e-5) + 4 * 65 * 2.0 ** -23 * absv
+        worst = float(((out.cpu().double() - want).abs() / tol).max())
+        print(f"window {window}: worst error / bound {worst:.3f}")
+        assert worst <= 1.0
+    assert E.kernel_status(0) == 0
