@@ -442,10 +442,11 @@ __global__ void __launch_bounds__(Page::WARPS * 32)
       L += f * wl[w * kMaxGroup + h];
       O += f * wo[w * kMaxGroup * D + i];
     }
-    if (C == 1 && !any_failed) out[i] = Elem<T>::from_f(L > 0.f ? O / L : 0.f);
+    // (a row that sees no key has L = 0; a NaN that it sees makes L NaN, and its result)
+    if (C == 1 && !any_failed) out[i] = Elem<T>::from_f(L == 0.f ? 0.f : O / L);
     co[i] = O;
     if (i % D == 0) {
-      cm[h] = any_failed ? NAN : M;  // a NaN maximum tells the cluster that a wait ran out
+      cm[h] = any_failed ? NAN : M;  // a NaN maximum tells the cluster that a wait ran out (fmaxf gives none)
       cl[h] = L;
     }
   }
@@ -484,7 +485,7 @@ __global__ void __launch_bounds__(Page::WARPS * 32)
         L += f * tl[c * kMaxGroup + t];
       }
       wm[t] = bad ? NAN : M;
-      wl[t] = L > 0.f ? 1.f / L : 0.f;
+      wl[t] = L == 0.f ? 0.f : 1.f / L;
     }
     __syncthreads();
   }

@@ -144,3 +144,56 @@ def test_chunks_whose_scores_climb(name, step):
         print(f"window {window}: worst error / bound {worst:.3f}")
         assert worst <= 1.0
     assert E.kernel_status(0) == 0
+
+
+def same_nans(got, want, other, tol):
+    """NaN exactly where the formula has it; elsewhere within tol of it and the bits of `other`."""
+    got, nan = got.cpu(), want.isnan()
+    assert torch.equal(got.isnan(), nan)
+    assert torch.equal(got[~nan], other.cpu()[~nan])
+    assert bool(((got.double() - want).abs()[~nan] <= tol[~nan]).all())
+
+
+@pytest.mark.parametrize("name", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("window", [32, 2000])  # one CTA a row, a cluster
+@pytest.mark.parametrize("where", ["query", "key", "first key", "value", "infinite query"])
+def test_rows_that_see_a_nan(name, window, where):
+    dt, d, hkv, group = DTYPES[name], 64, 2, 2
+    g = torch.Generator().manual_seed(4)
+    ctx = [2500, 40, 2300, 1, 0]
+    rows, blocks = len(ctx), 160
+    k, v = (torch.randn(rows * blocks, hkv, 16, d, generator=g).to(dt) for _ in range(2))
+    tables = torch.arange(rows * blocks, dtype=torch.int32).reshape(rows, blocks)
+    rt = torch.arange(rows, dtype=torch.int32)
+    q = torch.randn(rows, hkv * group, d, generator=g).to(dt)
+    clean = torch.full(q.shape, 5.0, dtype=dt, device=DEV)
+    sync_ok(run_rows(q, k, v, tables, rt, ctx, window, 0, clean))
+    w_clean = torch.zeros(rows, hkv, 2500, device=DEV)
+    sync_ok(run_weights(q.to(DEV), k.to(DEV), v.to(DEV), tables.to(DEV), rt.to(DEV), ctx, torch.empty_like(clean), w_clean))
+    for row in range(3 if where == "infinite query" else 4):  # (one key's score alone may be -infinity)
+        qq, kk, vv = q.clone(), k.clone(), v.clone()
+        at = ctx[row] - 1 if where != "first key" else max(0, ctx[row] - window)
+        page = int(tables[row, at // 16])
+        if where == "query":
+            qq[row, 1, 7] = math.nan
+        elif where == "infinite query":
+            qq[row, 1, 7] = math.inf  # scores of both signs: infinity less infinity
+        elif where == "value":
+            vv[page, 0, at % 16, 9] = math.nan
+        else:
+            kk[page, 0, at % 16, 9] = math.nan
+        out = torch.full(q.shape, 5.0, dtype=dt, device=DEV)
+        sync_ok(run_rows(qq, kk, vv, tables, rt, ctx, window, 0, out))
+        want, _, absv, smax = ref.window_rows(qq, kk, vv, tables, rt, ctx, window, 0, ref.scale_of(d))
+        assert want.isnan().any()
+        same_nans(out, want, clean, ref.bound(dt, want, absv, smax, max(ctx), d))
+        # every key of a head whose sum is NaN gets NaN, no other key does
+        w, o = torch.zeros_like(w_clean), torch.full(q.shape, 5.0, dtype=dt, device=DEV)
+        sync_ok(run_weights(qq.to(DEV), kk.to(DEV), vv.to(DEV), tables.to(DEV), rt.to(DEV), ctx, o, w))
+        want, add, _, _ = ref.window_rows(qq, kk, vv, tables, rt, ctx, 0, 0, ref.scale_of(d))
+        assert torch.equal(o.cpu().isnan(), want.isnan())
+        for r, n in enumerate(ctx):
+            nan = add[r].isnan()
+            got, base = w[r, :, :n].cpu(), w_clean[r, :, :n].cpu()
+            assert torch.equal(got.isnan(), nan) and torch.equal(got[~nan], base[~nan])
+    assert E.kernel_status(0) == 0
