@@ -216,10 +216,12 @@ __device__ __forceinline__ void cp_async_arrive_on(uint64_t *bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
-// max of three (sm_100 three-input max.f32)
-__device__ __forceinline__ float max3f(float a, float b, float c) {
+// max of three (sm_100 three-input max.f32).  With KEEP_NAN a NaN among them is the result, else
+// it is passed over.
+template <bool KEEP_NAN> __device__ __forceinline__ float max3f(float a, float b, float c) {
   float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  if constexpr (KEEP_NAN) asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  else asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 // 2^x for two x <= 15 on the FMA and integer pipes instead of the transcendental unit
@@ -490,7 +492,7 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
           auto chunk_max = [&](auto m) {
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-              mx[i & 3] = max3f(mx[i & 3], score(m, cur, k, 2 * i, bits), score(m, cur, k, 2 * i + 1, bits));
+              mx[i & 3] = max3f<WIN>(mx[i & 3], score(m, cur, k, 2 * i, bits), score(m, cur, k, 2 * i + 1, bits));
           };
           // a masked group's chunks are mostly seen whole by a warp's rows: no select for those
           if constexpr (WIN && decltype(masked)::value) {
@@ -500,14 +502,18 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
             chunk_max(masked);
           }
         }
-        return fmaxf(max3f(mx[0], mx[1], mx[2]), mx[3]);
+        const float m = max3f<WIN>(mx[0], mx[1], mx[2]);
+        return WIN ? max3f<WIN>(m, mx[3], mx[3]) : fmaxf(m, mx[3]);
       };
       const float mt = diag ? row_max(std::true_type{}) : row_max(std::false_type{});
       const float mts = mt * c;
-      const bool grow = mts > m_run + Reference<T, WIN>::kGrow;  // m_run = -inf: any finite max
+      // m_run = -inf: any finite max.  Windowed build: a maximum of NaN or infinity makes the
+      // reference NaN, and with it the row (the polynomial's clamp would pass over a NaN score).
+      const float limit = m_run + Reference<T, WIN>::kGrow;
+      const bool grow = WIN ? !(mts <= limit) : mts > limit;
       float alpha = 1.f;
       if (grow) {
-        const float m_new = mts - Reference<T, WIN>::kDrop;
+        const float m_new = WIN && !(mts < INFINITY) ? NAN : mts - Reference<T, WIN>::kDrop;
         alpha = ex2_approx(m_run - m_new);
         m_run = m_new;
       }
@@ -753,8 +759,8 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
     constexpr int NCH = D / 4;  // 16-byte chunks per row
     if (warp < 4 * kHalves) {
       const int r = qh * kRows + rt;
-      rm[r] = all_ok ? m_run : NAN;  // a NaN tells the cluster that a wait ran out
-      rl[r] = l_run;
+      rm[r] = m_run;
+      rl[r] = all_ok ? l_run : -1.f;  // a sum below 0 tells the cluster that a wait ran out
       if (all_ok && ng_q > 0) {
         const uint32_t tm_o = tmem + qh * 256 + kKeys + (uint32_t((warp & 3) * 32) << 16);
 #pragma unroll
@@ -770,7 +776,8 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
     }
     if (!all_ok && t == 0) atomicOr(p.status, kStatusWaitTimeout);
     cluster_sync();
-    // weights of the shares, once per row: 2^(m_s - M) / L, 0 for a share that saw nothing
+    // weights of the shares, once per row: 2^(m_s - M) / L, 0 for a share that saw nothing, -1
+    // where a wait ran out
     float *rw = rl + kHalves * kRows;  // [8][256], this CTA's rows by their place among them
     for (int i = t; int(blockIdx.z) + p.splits * i < kHalves * kRows; i += kThreads5) {
       const int r = int(blockIdx.z) + p.splits * i;
@@ -783,7 +790,7 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
       }
 #pragma unroll
       for (int s = 0; s < 8; ++s) {
-        bad |= m[s] != m[s];
+        bad |= l[s] < 0.f;
         M = fmaxf(M, m[s]);
       }
 #pragma unroll
@@ -791,10 +798,10 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
         m[s] = m[s] == -INFINITY ? 0.f : ex2_approx(m[s] - M);
         L += m[s] * l[s];
       }
-      const float inv = bad ? NAN : L > 0.f ? 1.f / L : 0.f;
+      const float inv = L == 0.f ? 0.f : 1.f / L;
 #pragma unroll
       for (int s = 0; s < 8; ++s)
-        if (s < p.splits) rw[s * 256 + i] = m[s] == 0.f && !bad ? 0.f : m[s] * inv;
+        if (s < p.splits) rw[s * 256 + i] = bad ? -1.f : m[s] == 0.f ? 0.f : m[s] * inv;
     }
     __syncthreads();
     // A thread per 16-byte chunk of a row (whole rows per request, no bank conflicts), every
@@ -819,7 +826,7 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
         o[2] += f * __uint_as_float(u[s].z);
         o[3] += f * __uint_as_float(u[s].w);
       }
-      if (rw[i] != rw[i]) continue;  // a wait ran out
+      if (rw[i] < 0.f) continue;  // a wait ran out
       *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) +
                                  ((size_t(row0) + tk) * p.num_kv_heads * G + size_t(kvh) * G + hd) * D + ch * 4) =
           make_uint2(pack_pair<T>(o[0], o[1]), pack_pair<T>(o[2], o[3]));
@@ -833,7 +840,7 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
       // TMEM loads.
       const uint32_t lane_off = uint32_t((warp & 3) * 32) << 16;
       const uint32_t tm_o = tmem + qh * 256 + kKeys;
-      const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+      const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
       unsigned char *stage = sq + size_t(warp * 32) * (D * 2);
 #pragma unroll
       for (int c0 = 0; c0 < D; c0 += 32) {

@@ -197,3 +197,47 @@ def test_rows_that_see_a_nan(name, window, where):
             got, base = w[r, :, :n].cpu(), w_clean[r, :, :n].cpu()
             assert torch.equal(got.isnan(), nan) and torch.equal(got[~nan], base[~nan])
     assert E.kernel_status(0) == 0
+
+
+@pytest.mark.parametrize("name,group,hkv,d", [("bf16", 2, 2, 64), ("f16", 1, 2, 128)])
+@pytest.mark.parametrize("window", [300, 2600])  # one CTA a tile, a cluster
+def test_chunks_that_see_a_nan(name, group, hkv, d, window):
+    dt, start, rows = DTYPES[name], 3000, 150
+    g = torch.Generator().manual_seed(4)
+    n = start + rows
+    k, v = (torch.randn(n, hkv, d, generator=g).to(dt) for _ in range(2))
+    q = torch.randn(rows, hkv * group, d, generator=g).to(dt)
+    kp, vp, tables, rt = one_sequence(k, v)
+    tl = tiles_of([(start, rows)], rt, group)
+
+    def go(q, kp, vp):
+        out = torch.full(q.shape, 5.0, dtype=dt, device=DEV)
+        sync_ok(run_chunk(q, kp, vp, tables, tl, window, 0, out))
+        return out
+
+    def want(q, kp, vp):
+        return ref.window_rows(q, kp, vp, tables, rt.expand(rows), [start + i + 1 for i in range(rows)], window, 0,
+                               ref.scale_of(d))
+
+    clean = go(q, kp, vp)
+    base, _, absv, smax = want(q, kp, vp)
+    tol = ref.bound(dt, base, absv, smax, n, d, exp_err=8e-5)
+    assert bool(((clean.cpu().double() - base).abs() <= tol).all())
+    for row in (0, 77, rows - 1):
+        for bad in (math.nan, math.inf):
+            qq = q.clone()
+            qq[row, 1, 3] = bad
+            exp = base.clone()
+            exp[row, 1] = math.nan
+            same_nans(go(qq, kp, vp), exp, clean, tol)
+    # a key of each of 16 columns next to one another, seen by all rows and by some
+    for key in [*range(start - 130, start - 114), start, start + 20, n - 1, start - window + 3]:
+        kk = kp.clone()
+        kk[int(tables[0, key // 16]), 0, key % 16, 5] = math.nan
+        exp = base.clone()
+        for i in range(rows):
+            if key <= start + i and start + i - key < window:
+                exp[i, :group] = math.nan
+        got = go(q, kk, vp)
+        same_nans(got, exp, clean, tol)
+    assert E.kernel_status(0) == 0
