@@ -447,7 +447,12 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
       lo_last = VisiblePages::lowest_key(pos0 + min(nrows, (qh + 1) * TPH) - 1, p.window) + shift;
       if (lo_last <= p.sinks) lo_last = 0;
     }
-    const float c = p.qscale;
+    // m_run is the row's reference in base 2, m_p what is taken from a score times c.  m is a rounded
+    // product, the FMA's s c is exact: every P of the row carries 2^(half a step of m), which the sum
+    // shares.  From |m| > 2^22 on (where f32 scores hold no fraction worth the name) that could leave
+    // P's range, so such a row goes on with c rounded down to a power of two, which makes both exact.
+    constexpr float kHuge = 4194304.f;
+    float c = p.qscale, m_p = 0.f, limit = -INFINITY;  // limit: the largest maximum that m_p serves
     // the lowest half that attends to the last group zeroes its V rows past the sequence
     const bool zeroes_v = qh == 0 ? last_half0 : last_half1 && !last_half0;
     for (int g = 0; g < ng_q; ++g) {
@@ -507,13 +512,23 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
       };
       const float mt = diag ? row_max(std::true_type{}) : row_max(std::false_type{});
       const float mts = mt * c;
-      // m_run = -inf: any finite max.  Windowed build: a maximum of NaN or infinity makes the
-      // reference NaN, and with it the row (the polynomial's clamp would pass over a NaN score).
-      const float limit = m_run + Reference<T, WIN>::kGrow;
-      const bool grow = WIN ? !(mts <= limit) : mts > limit;
+      const bool grow = WIN ? !(mts <= limit) : mts > m_run + Reference<T, WIN>::kGrow;  // m_run = -inf: any finite max
       float alpha = 1.f;
       if (grow) {
-        const float m_new = WIN && !(mts < INFINITY) ? NAN : mts - Reference<T, WIN>::kDrop;
+        float m_new = mts;
+        if constexpr (WIN) {
+          c = p.qscale;
+          m_p = m_new = mt * c - Reference<T, WIN>::kDrop;
+          limit = m_new + Reference<T, WIN>::kGrow;
+          if (!(fabsf(m_new) <= kHuge)) {
+            // a maximum of NaN or infinity makes the reference NaN, and with it the row (the
+            // polynomial's clamp would pass over a NaN score)
+            const float top = mt < INFINITY ? mt : NAN;
+            m_new = top * c;
+            c = __uint_as_float(__float_as_uint(p.qscale) & 0x7f800000u);
+            m_p = limit = top * c;
+          }
+        }
         alpha = ex2_approx(m_run - m_new);
         m_run = m_new;
       }
@@ -533,8 +548,8 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
           tmem_st32(tm_o + lane_off + c0, o);
         }
       }
-      // a windowed row may have seen nothing yet: -inf scores then give 2^-inf = 0
-      const float negm = WIN && m_run == -INFINITY ? 0.f : -m_run;
+      // a windowed row may have seen nothing yet (m_p = 0): -inf scores then give 2^-inf = 0
+      const float negm = WIN ? -m_p : -m_run;
       float ps[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       // P of chunk k (16 columns of value pairs) goes to columns [16k, 16k + 16): over S chunks
       // already read, never over the chunk loading next.  Two scores per packed FMA and add.

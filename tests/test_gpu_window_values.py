@@ -241,3 +241,52 @@ def test_chunks_that_see_a_nan(name, group, hkv, d, window):
         got = go(q, kk, vp)
         same_nans(got, exp, clean, tol)
     assert E.kernel_status(0) == 0
+
+
+@pytest.mark.parametrize("name,group,hkv,d", [("bf16", 2, 2, 64), ("bf16", 1, 2, 128)])
+@pytest.mark.parametrize("window", [300, 2600])  # one CTA a tile, a cluster
+def test_chunks_of_huge_scores(name, group, hkv, d, window):
+    """Finite scores of any size: the key that is ahead takes the row, the ones behind have no part."""
+    dt, start, rows = DTYPES[name], 3000, 150
+    g = torch.Generator().manual_seed(4)
+    n = start + rows
+    k, v = (torch.randn(n, hkv, d, generator=g).to(dt) for _ in range(2))
+    q = torch.randn(rows, hkv * group, d, generator=g).to(dt)
+    kp, vp, tables, rt = one_sequence(k, v)
+    tl = tiles_of([(start, rows)], rt, group)
+
+    def go(q, kp, vp):
+        out = torch.full(q.shape, 5.0, dtype=dt, device=DEV)
+        sync_ok(run_chunk(q, kp, vp, tables, tl, window, 0, out))
+        return out
+
+    # finite numbers whose product is infinite (not in f16: its products fit f32)
+    for key in range(start - 130, start - 126):
+        qq, kk = q.clone(), kp.clone()
+        qq[40, 0, 5], kk[int(tables[0, key // 16]), 0, key % 16, 5] = 1e30, 1e30
+        got = go(qq, kk, vp)
+        assert got[40, 0].isnan().all() and not got[41].isnan().any()
+    compared = 0
+    # one key of each of 16 neighbouring columns, many keys (each a multiple of the last), all keys
+    for size in (1e5, 3e7, 1e12, 1e30):
+        for keys in [[start - 130 + i] for i in range(16)] + [list(range(start - 200, start, 16)), list(range(0, start - 20))]:
+            kk = kp.clone()
+            for i, key in enumerate(keys):
+                kk[int(tables[0, key // 16]), 0, key % 16, 5] = size * (1 + i % 7) * (1 if len(keys) < 100 else -1)
+            got = go(q, kk, vp).cpu().double()
+            assert torch.isfinite(got).all()
+            # Rows whose largest score stands 2^-14 of its size before the next (f32 scores are good to
+            # d 2^-23 of it) are one value, rounded once with a weight rounded once.
+            half = torch.finfo(dt).eps / 2
+            pos, at = torch.arange(start, n)[:, None], torch.arange(n)[None]
+            seen = (at <= pos) & (pos - at < window)
+            for h in range(group):
+                s = (q[:, h].double() @ ref.paged(kk, tables[0], 0, n).double().T * ref.scale_of(d)).masked_fill(~seen, -math.inf)
+                top = s.topk(2, -1)
+                ahead = top.values[:, 0] - top.values[:, 1] > (2.0 ** -14 * s.masked_fill(~seen, 0).abs().amax(-1)).clamp(min=60.0)
+                val = ref.paged(vp, tables[0], 0, n).double()[top.indices[:, 0]]
+                off = (got[:, h] - val).abs() <= 2.02 * half * val.abs() + 1e-30
+                assert bool(off[ahead].all()), (size, keys[:2], h)
+                compared += int(ahead.sum())
+    assert compared > 1000
+    assert E.kernel_status(0) == 0
