@@ -34,6 +34,7 @@
 // them back once the cluster has exchanged the maxima and sums.
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
 #include <type_traits>
 
 #include "ms_window.cuh"
@@ -44,6 +45,9 @@ namespace {
 using namespace attn;
 
 constexpr int kMaxCluster = 8;
+// running maxima start here, not at -infinity: a page whose scores are all -infinity (products below
+// the f32 range) then gives 2^-infinity = 0 and no NaN
+constexpr float kLowest = -FLT_MAX;
 
 struct RowsParams {
   const void *q, *k_pool, *v_pool;
@@ -71,7 +75,7 @@ template <typename T_, int D_> struct PageTc {
   static constexpr float kScaleP = std::is_same<T, __half>::value ? 32768.f : 1.f;
   uint32_t qa[KSTEPS][2];
   float o[NTD][4];
-  float m_run = -INFINITY, l_run = 0.f;
+  float m_run = kLowest, l_run = 0.f;
 
   __device__ __forceinline__ void init(const T *q, int group, float) {
     const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
@@ -202,7 +206,7 @@ template <int D_, int G> struct PageF32 {
 #pragma unroll
     for (int h = 0; h < G; ++h) {
       TileLoad<float, D>::load(q + h * D, lane, qv[h]);
-      m_run[h] = -INFINITY;
+      m_run[h] = kLowest;
 #pragma unroll
       for (int d = 0; d < DPL; ++d) {
         qv[h][d] *= qscale;
@@ -438,7 +442,7 @@ __global__ void __launch_bounds__(Page::WARPS * 32)
     for (int w = 0; w < W; ++w) M = fmaxf(M, wm[w * kMaxGroup + h]);
 #pragma unroll
     for (int w = 0; w < W; ++w) {
-      const float mw = wm[w * kMaxGroup + h], f = mw == -INFINITY ? 0.f : exp2f(mw - M);
+      const float f = exp2f(wm[w * kMaxGroup + h] - M);
       L += f * wl[w * kMaxGroup + h];
       O += f * wo[w * kMaxGroup * D + i];
     }
@@ -480,7 +484,7 @@ __global__ void __launch_bounds__(Page::WARPS * 32)
         M = fmaxf(M, mc);
       }
       for (int c = 0; c < C; ++c) {
-        const float mc = tm[c * kMaxGroup + t], f = mc == -INFINITY ? 0.f : exp2f(mc - M);
+        const float f = exp2f(tm[c * kMaxGroup + t] - M);
         tf[c * kMaxGroup + t] = f;
         L += f * tl[c * kMaxGroup + t];
       }

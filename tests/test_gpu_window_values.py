@@ -290,3 +290,39 @@ def test_chunks_of_huge_scores(name, group, hkv, d, window):
                 compared += int(ahead.sum())
     assert compared > 1000
     assert E.kernel_status(0) == 0
+
+
+@pytest.mark.parametrize("name", ["bf16", "f32"])
+@pytest.mark.parametrize("window", [60, 2000])  # one CTA a row, a cluster
+def test_scores_of_minus_infinity_have_no_weight(name, window):
+    """Finite keys whose product with the query is below the f32 range: weight 0, whole pages of
+    them too, wherever they lie."""
+    dt, d, n = DTYPES[name], 64, 2100
+    g = torch.Generator().manual_seed(6)
+    k, v = (torch.randn(n, 1, d, generator=g).to(dt) for _ in range(2))
+    q = torch.randn(1, 2, d, generator=g).to(dt)
+    q[..., 5] = 1e3
+    k[..., 5] = 0.0
+    for keys in (range(n - 60, n - 30), range(n - 20, n), range(0, n - 30), [n - 1], range(n - 40, n, 2)):
+        kk = k.clone()
+        kk[list(keys), :, 5] = -3e38
+        kp, vp, tables, rt = one_sequence(kk, v)
+        out = torch.full(q.shape, math.nan, dtype=dt, device=DEV)
+        sync_ok(run_rows(q, kp, vp, tables, rt, [n], window, 0, out))
+        # the reference without those keys' huge components: a score 10^4 below all others
+        kk[list(keys), :, 5] = -80.0
+        kp2 = one_sequence(kk, v)[0]
+        want, _, absv, smax = ref.window_rows(q, kp2, vp, tables, rt, [n], window, 0, ref.scale_of(d))
+        tol = ref.bound(dt, want, absv, torch.full_like(smax, 100.0), n, d)
+        assert bool(((out.cpu().double() - want).abs() <= tol).all()), keys
+        want, add, absv, smax = ref.window_rows(q, kp2, vp, tables, rt, [n], 0, 0, ref.scale_of(d))
+        w = torch.zeros(1, 1, n, device=DEV)
+        sync_ok(run_weights(q.to(DEV), kp.to(DEV), vp.to(DEV), tables.to(DEV), rt.to(DEV), [n], out, w))
+        assert bool(((out.cpu().double() - want).abs() <= tol).all()), keys
+        assert float((w[0].cpu().double() - add[0]).abs().max()) < 1e-4
+        assert (w[0, 0, list(keys)] == 0).all()
+        if dt != torch.float32:
+            o = torch.full(q.shape, math.nan, dtype=dt, device=DEV)
+            sync_ok(run_chunk(q, kp, vp, tables, tiles_of([(n - 1, 1)], rt, 2), 0, 0, o))
+            assert bool(((o.cpu().double() - want).abs() <= tol + 2e-4 * absv).all()), keys
+    assert E.kernel_status(0) == 0
