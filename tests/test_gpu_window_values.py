@@ -326,3 +326,44 @@ def test_scores_of_minus_infinity_have_no_weight(name, window):
             sync_ok(run_chunk(q, kp, vp, tables, tiles_of([(n - 1, 1)], rt, 2), 0, 0, o))
             assert bool(((o.cpu().double() - want).abs() <= tol + 2e-4 * absv).all()), keys
     assert E.kernel_status(0) == 0
+
+
+@pytest.mark.parametrize("name", ["bf16", "f16", "f32"])
+def test_large_numbers_that_no_row_sees(name):
+    """Keys and values between the sinks and the window, on pages that hold seen keys too, change no bit."""
+    dt, d, n, window, sinks = DTYPES[name], 128, 90, 40, 3
+    g = torch.Generator().manual_seed(1)
+    k, v = (torch.randn(n, 2, d, generator=g).to(dt) for _ in range(2))
+    q = torch.randn(5, 4, d, generator=g).to(dt)
+    big = torch.finfo(dt).max
+
+    def go(k, v, first):
+        kp, vp, tables, rt = one_sequence(k, v)
+        out = torch.full(q.shape, math.nan, dtype=dt, device=DEV)
+        if first == n - 1:
+            sync_ok(run_rows(q[:1], kp, vp, tables, rt, [n], window, sinks, out))
+            return out[:1]
+        tl = tiles_of([(first, n - first)], rt, 2)
+        sync_ok(run_chunk(q, kp, vp, tables, tl, window, sinks, out))
+        return out
+
+    for first in [n - 1] + ([n - 5] if dt != torch.float32 else []):  # the row at n - 1; the rows from n - 5 on
+        base = go(k, v, first)
+        low = first + 1 - window  # the first key of the first row's window
+        assert torch.isfinite(base).all() and low > 40
+        for at in (3, 15, 16, 30, 40, low - 1):
+            for sign in (1, -1):
+                kk, vv = k.clone(), v.clone()
+                kk[at], vv[at] = sign * big, -sign * big
+                assert torch.equal(go(kk, vv, first), base), (first, at)
+    # keys that the chunk's first rows see and its last do not, and the other way round
+    if dt != torch.float32:
+        first = n - 5
+        base = go(k, v, first)
+        for at, sees in ((first + 1 - window, [0]), (n - 2, [3, 4])):
+            vv = v.clone()
+            vv[at] = big
+            got = go(k, vv, first)
+            for r in range(5):
+                assert torch.equal(got[r], base[r]) == (r not in sees), (at, r)
+    assert E.kernel_status(0) == 0
