@@ -296,7 +296,8 @@ int ms_engine_graph_stats(const ms_engine *eng, int64_t *captures, int64_t *repl
  * of later steps the token at position p attends to the keys j <= p with
  * p - j < window or j < sinks (ms_launch_window_attention and
  * ms_launch_window_prefill); window = 0 restores full attention.  Block
- * tables still cover the whole sequence.  Drops the captured graphs; under
+ * tables still cover the whole sequence.  first_layer is at most the layer
+ * count (no layer has the window then).  Drops the captured graphs; under
  * tensor parallelism every rank makes the same call between the same steps. */
 int ms_engine_set_window(ms_engine *eng, int32_t window, int32_t sinks, int32_t first_layer);
 

@@ -239,7 +239,8 @@ class Engine:
             raise error_for(rc, "ms_engine_create: " + self._err(None))
         self.h = h
         if getattr(cfg, "sliding_window", None):
-            self.set_window(cfg.sliding_window, 0, getattr(cfg, "max_window_layers", 0))
+            # (a configuration may name more layers than the model has: then none has the window)
+            self.set_window(cfg.sliding_window, 0, min(getattr(cfg, "max_window_layers", 0), cfg.num_hidden_layers))
         self._out_tok = np.zeros(max_seqs, np.uint32)
         self._out_flags = np.zeros(max_seqs, np.uint8)
 
