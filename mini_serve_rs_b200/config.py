@@ -23,6 +23,7 @@ class ModelConfig:
     # keys a token attends to in layers >= max_window_layers; None: the whole context
     sliding_window: Optional[int] = None
     max_window_layers: int = 0
+    use_sliding_window: bool = True  # false: sliding_window is set but not used (Qwen2 configurations)
 
     def hd(self) -> int:
         return self.head_dim or self.hidden_size // self.num_attention_heads

@@ -218,7 +218,8 @@ class Engine:
         hidden_size, intermediate_size, num_hidden_layers, num_attention_heads,
         num_key_value_heads, head_dim or hd(), max_position_embeddings,
         rope_theta, rms_norm_eps, qk_norm, attention_bias, tie_word_embeddings);
-        where it has a sliding_window, layers from its max_window_layers on use it."""
+        where it has a sliding_window, layers from its max_window_layers on use it
+        unless its use_sliding_window is false."""
         self.lib = lib()
         self.cfg = cfg
         hd = cfg.hd() if hasattr(cfg, "hd") else cfg.head_dim
@@ -238,7 +239,7 @@ class Engine:
         if rc != MS_OK:
             raise error_for(rc, "ms_engine_create: " + self._err(None))
         self.h = h
-        if getattr(cfg, "sliding_window", None):
+        if getattr(cfg, "sliding_window", None) and getattr(cfg, "use_sliding_window", True):
             # (a configuration may name more layers than the model has: then none has the window)
             self.set_window(cfg.sliding_window, 0, min(getattr(cfg, "max_window_layers", 0), cfg.num_hidden_layers))
         self._out_tok = np.zeros(max_seqs, np.uint32)

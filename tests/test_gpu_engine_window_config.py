@@ -42,3 +42,11 @@ def test_no_layer_from_max_window_layers_on(first):
     """max_window_layers at or above the layer count: no layer has the window."""
     cfg = dataclasses.replace(CFG, sliding_window=30, max_window_layers=first)
     assert np.array_equal(logits(cfg), logits(CFG))
+
+
+def test_use_sliding_window_off():
+    cfg = dataclasses.replace(CFG, sliding_window=30, max_window_layers=1, use_sliding_window=False)
+    assert np.array_equal(logits(cfg), logits(CFG))
+    on = dataclasses.replace(cfg, use_sliding_window=True)
+    assert np.array_equal(logits(on), logits(CFG, [(30, 0, 1)]))
+    assert not np.array_equal(logits(on), logits(CFG))
