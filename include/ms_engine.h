@@ -171,7 +171,8 @@ int ms_nccl_comm_destroy(void *comm);
 
 /* Admit a sequence (scheduler.rs:347-369): its prompt tokens and the logical
  * KV blocks KVCache::allocate returned (kv_cache.rs:61-84).  num_cached
- * prompt tokens already have their K/V in those blocks (a shared prefix);
+ * prompt tokens already have their K/V in those blocks (a shared prefix,
+ * computed under the sliding window set now: MS_E_INVALID otherwise);
  * when num_cached == prompt length the last prompt token is replayed, as the
  * reference does on an exact prefix hit without logits (candle.rs:447-455). */
 int ms_seq_admit(ms_engine *eng, uint64_t seq_id, const uint32_t *prompt, int32_t prompt_len,
@@ -298,7 +299,11 @@ int ms_engine_graph_stats(const ms_engine *eng, int64_t *captures, int64_t *repl
  * ms_launch_window_prefill); window = 0 restores full attention.  Block
  * tables still cover the whole sequence.  first_layer is at most the layer
  * count (no layer has the window then).  Drops the captured graphs; under
- * tensor parallelism every rank makes the same call between the same steps. */
+ * tensor parallelism every rank makes the same call between the same steps.
+ * K/V in the pool stay as they were computed: admitted sequences go on over
+ * theirs, and ms_seq_admit refuses cached tokens on blocks that a step wrote
+ * under another window, so a prefix cache filled before the call has to be
+ * emptied (a new ms_pages). */
 int ms_engine_set_window(ms_engine *eng, int32_t window, int32_t sinks, int32_t first_layer);
 
 /* Tensor parallelism: *fused = 1 when the all-reduces after o_proj and

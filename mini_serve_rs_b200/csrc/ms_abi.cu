@@ -2,6 +2,7 @@
 // Every entry point catches C++ exceptions and turns them into status codes.
 #include <cstring>
 #include <algorithm>
+#include <array>
 #include <exception>
 #include <new>
 #include <string>
@@ -219,13 +220,24 @@ extern "C" int ms_engine_set_window(ms_engine *eng, int32_t window, int32_t sink
   if (window < 0 || sinks < 0 || first_layer < 0 || first_layer > eng->L)
     return eng->fail(MS_E_INVALID, "window and sinks must not be negative, first_layer within the layers");
   if (window == eng->window && sinks == eng->window_sinks && first_layer == eng->window_layer0) return MS_OK;
-  cudaSetDevice(eng->dev);
-  cudaStreamSynchronize(eng->stream);
-  eng->drop_graphs();  // captured with the old window
-  eng->window = window;
-  eng->window_sinks = sinks;
-  eng->window_layer0 = first_layer;
-  return MS_OK;
+  return guarded(eng, [&] {
+    // a window that hides no key of a full block table, or from no layer, is no window
+    const bool binds = window > 0 && first_layer < eng->L &&
+                       int64_t(window) + sinks < int64_t(eng->opts.max_blocks_per_seq) * eng->opts.block_size;
+    const std::array<int, 3> setting =
+        binds ? std::array<int, 3>{window, sinks, first_layer} : std::array<int, 3>{0, 0, 0};
+    auto &known = eng->window_settings;
+    auto it = std::find(known.begin(), known.end(), setting);
+    if (it == known.end()) it = known.insert(known.end(), setting);
+    cudaSetDevice(eng->dev);
+    cudaStreamSynchronize(eng->stream);
+    eng->drop_graphs();  // captured with the old window
+    eng->window_setting = int32_t(it - known.begin());
+    eng->window = window;
+    eng->window_sinks = sinks;
+    eng->window_layer0 = first_layer;
+    return MS_OK;
+  });
 }
 
 extern "C" int ms_engine_set_graphs(ms_engine *eng, int32_t on) {

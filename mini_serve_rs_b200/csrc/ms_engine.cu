@@ -176,6 +176,7 @@ int create_impl(const ms_model_cfg *cfg, const ms_engine_opts *opts, Engine *eng
   eng->layer_pool_elems = size_t(opts->pool_blocks) * eng->hkv * 16 * D;
   eng->pool_bytes = eng->layer_pool_elems * 2 * eng->L * es;
   MS_CUDA_TRY(cudaMalloc(&eng->pool, eng->pool_bytes));
+  eng->page_window.assign(size_t(opts->pool_blocks), Engine::kPageUnwritten);
 
   // ---- tensor maps for the tensor-core attention kernels ----
   eng->use_tc = attention_tc_available(eng->dtype, eng->D, eng->hq / eng->hkv);

@@ -5,6 +5,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <array>
 #include <string>
 #include <unordered_map>
 #include <vector>
@@ -73,6 +74,19 @@ struct Engine {
   // sliding window of layers >= window_layer0 (ms_engine_set_window); 0: full attention
   int window = 0, window_sinks = 0, window_layer0 = 0;
   bool windowed(int layer) const { return window > 0 && layer >= window_layer0; }
+  // The setting that each page's K/V were computed under, as an index into window_settings, so that
+  // ms_seq_admit does not share a prefix across a change of the window
+  static constexpr int32_t kPageUnwritten = -1, kPageMixed = -2;  // by no step; by steps of several settings
+  std::vector<std::array<int, 3>> window_settings{{0, 0, 0}};
+  int32_t window_setting = 0;
+  std::vector<int32_t> page_window;  // [pool_blocks]
+  void mark_written(const std::vector<int32_t> &blocks, int start, int end) {
+    for (int b = start / opts.block_size; b * opts.block_size < end; ++b) {
+      int32_t &w = page_window[blocks[b]];
+      if (b * opts.block_size >= start || w == kPageUnwritten) w = window_setting;
+      else if (w != window_setting) w = kPageMixed;
+    }
+  }
 
   // per-slot device state
   int32_t *d_block_tables = nullptr;  // [max_seqs][max_blocks_per_seq]

@@ -31,6 +31,12 @@ int seq_admit_impl(Engine *eng, uint64_t id, const uint32_t *prompt, int prompt_
   for (int i = 0; i < nblocks; ++i)
     if (blocks[i] < 0 || blocks[i] >= eng->opts.pool_blocks)
       return eng->fail(MS_E_INVALID, "block id " + std::to_string(blocks[i]) + " outside the pool");
+  for (int i = 0; i * eng->opts.block_size < num_cached; ++i) {
+    const int32_t w = eng->page_window[blocks[i]];
+    if (w != Engine::kPageUnwritten && w != eng->window_setting)
+      return eng->fail(MS_E_INVALID, "cached block " + std::to_string(blocks[i]) +
+                                         " was computed under another sliding window");
+  }
   for (int i = 0; i < prompt_len; ++i)
     if (prompt[i] >= uint32_t(eng->V)) return eng->fail(MS_E_INVALID, "prompt token outside the vocabulary");
   if (eng->free_slots.empty()) return eng->fail(MS_E_PRESSURE, "no free sequence slot");

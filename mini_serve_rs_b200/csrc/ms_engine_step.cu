@@ -371,6 +371,7 @@ int step_launch_impl(Engine *eng, const ms_step_desc *desc) {
     if (r.partial) eng->last_flags[i] = MS_FLAG_NO_TOKEN;
     else if (r.prefill) eng->last_flags[i] = MS_FLAG_PREFILLED;
     eng->last_out_flags[r.orig] = eng->last_flags[i];
+    eng->mark_written(r.seq->blocks, r.start, r.start + r.ntok);
     r.seq->cached = r.start + r.ntok;
     if (!r.partial) r.seq->prefilled = true;
     r.seq->synced = int(r.seq->blocks.size());
