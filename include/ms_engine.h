@@ -435,7 +435,9 @@ int ms_prefill_tiles(const int32_t *seq_row0, const int32_t *seq_ntok, const int
  *  - k_pool / v_pool [pool_blocks, num_kv_heads, 16, head_dim], 16-byte
  *    aligned; block_tables [table_rows, max_blocks_per_seq]; num_heads /
  *    num_kv_heads is 1, 2, 4, 7 or 8, head_dim 64 or 128, block_size 16;
- *    q and out [rows, num_heads, head_dim], 16-byte aligned; scale > 0.
+ *    q and out [rows, num_heads, head_dim], 16-byte aligned; scale > 0.  All
+ *    other arrays are aligned as their elements, K3a's workspace to 16 bytes,
+ *    K7's to 4.
  *  - They run on the current device, allocate nothing, and may be captured
  *    into a graph; calls that may overlap need workspaces of their own.
  *  - Host arguments out of range return cudaErrorInvalidValue before anything

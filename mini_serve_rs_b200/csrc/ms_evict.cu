@@ -524,9 +524,10 @@ extern "C" int ms_launch_evict(void *k_pool, void *v_pool, int64_t pool_blocks, 
   if (!head_layout_ok(num_kv_heads, num_kv_heads, head_dim, block_size, dtype) || num_kv_heads > 65535 ||
       !pools_ok(k_pool, v_pool, pool_blocks, num_kv_heads, block_tables, table_rows, max_blocks_per_seq) ||
       max_ctx > kMaxCluster * kMaxSlots || max_ctx > int64_t(max_blocks_per_seq) * attn::kBS || stride < max_ctx ||
-      (!row_table && table_rows < num_rows) || !row_ctx || !row_next || (row_known && !pos_in) || !weight_in ||
-      !weight_out || !pos_out || keep <= 0 || sinks < 0 || recent < 0 || int64_t(sinks) + recent > keep ||
-      workspace == nullptr || workspace_bytes < evict_workspace_bytes(num_rows, num_kv_heads, max_ctx))
+      (row_table ? !ptr4(row_table) : table_rows < num_rows) || !ptr4(row_ctx) || !ptr4(row_next) ||
+      (row_known && (!ptr4(row_known) || !pos_in)) || (pos_in && !ptr4(pos_in)) || !ptr4(weight_in) ||
+      !ptr4(weight_out) || !ptr4(pos_out) || keep <= 0 || sinks < 0 || recent < 0 || int64_t(sinks) + recent > keep ||
+      !ptr4(workspace) || workspace_bytes < evict_workspace_bytes(num_rows, num_kv_heads, max_ctx))
     return int(cudaErrorInvalidValue);
   EvictParams p{};
   p.k_pool = static_cast<unsigned char *>(k_pool);

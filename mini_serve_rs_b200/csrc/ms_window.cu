@@ -673,12 +673,12 @@ bool common_ok(const WindowArgs &a) {
 cudaError_t launch_window_attention(const WindowArgs &a, cudaStream_t stream) {
   if (a.num_rows < 0 || a.max_ctx < 0) return cudaErrorInvalidValue;
   if (a.num_rows == 0) return cudaSuccess;
-  if (!common_ok(a) || !a.row_ctx || a.tiles || a.max_ctx > int64_t(a.max_blocks_per_seq) * attn::kBS ||
-      (!a.row_table && a.table_rows < a.num_rows))
+  if (!common_ok(a) || !ptr4(a.row_ctx) || a.tiles || a.max_ctx > int64_t(a.max_blocks_per_seq) * attn::kBS ||
+      (a.row_table ? !ptr4(a.row_table) : a.table_rows < a.num_rows))
     return cudaErrorInvalidValue;
   if (a.weight_sum) {
     const int64_t need = attention_weights_workspace_bytes(a.num_rows, a.num_heads, a.max_ctx);
-    if (a.row_index || a.weight_stride < a.max_ctx || (need > 0 && !ptr16(a.workspace)) || a.workspace_bytes < need)
+    if (a.row_index || !ptr4(a.weight_sum) || a.weight_stride < a.max_ctx || (need > 0 && !ptr16(a.workspace)) || a.workspace_bytes < need)
       return cudaErrorInvalidValue;
   }
   return launch_checked(a, stream);
@@ -688,7 +688,7 @@ cudaError_t launch_window_prefill(const WindowArgs &args, cudaStream_t stream) {
   WindowArgs a = args;
   if (a.num_tiles < 0) return cudaErrorInvalidValue;
   if (a.num_tiles == 0) return cudaSuccess;
-  if (!common_ok(a) || !a.tiles || a.dtype == MS_DTYPE_F32 || a.num_tiles > 65535) return cudaErrorInvalidValue;
+  if (!common_ok(a) || !ptr4(a.tiles) || a.dtype == MS_DTYPE_F32 || a.num_tiles > 65535) return cudaErrorInvalidValue;
   if (!attention_tc_available(a.dtype, a.head_dim, a.num_heads / a.num_kv_heads)) return cudaErrorInvalidValue;
   if (!a.status) {
     const cudaError_t e = standalone_status_word(&a.status);

@@ -89,10 +89,12 @@ inline bool head_layout_ok(int num_heads, int num_kv_heads, int head_dim, int bl
   return dtype == MS_DTYPE_F32 || dtype == MS_DTYPE_BF16 || dtype == MS_DTYPE_F16;
 }
 inline bool ptr16(const void *p) { return p != nullptr && reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+// 32-bit elements, as of tables, contexts, weights and positions
+inline bool ptr4(const void *p) { return p != nullptr && reinterpret_cast<uintptr_t>(p) % 4 == 0; }
 // pools and block tables of one call; 32-bit page x head tiles, as the TMA coordinates hold them
 inline bool pools_ok(const void *k_pool, const void *v_pool, int64_t pool_blocks, int num_kv_heads,
                      const int32_t *block_tables, int table_rows, int max_blocks_per_seq) {
-  return ptr16(k_pool) && ptr16(v_pool) && block_tables && pool_blocks > 0 && table_rows > 0 &&
+  return ptr16(k_pool) && ptr16(v_pool) && ptr4(block_tables) && pool_blocks > 0 && table_rows > 0 &&
          max_blocks_per_seq > 0 && max_blocks_per_seq <= (1 << 26) && num_kv_heads > 0 &&
          pool_blocks <= ((int64_t(1) << 31) - 1) / num_kv_heads;
 }
