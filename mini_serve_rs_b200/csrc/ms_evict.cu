@@ -30,6 +30,7 @@
 // moves' HBM traffic for many.
 #include <algorithm>
 #include <atomic>
+#include <cstddef>
 
 #include "ms_window.cuh"
 
@@ -71,7 +72,7 @@ __device__ __forceinline__ uint32_t rank_key(float w) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-struct Shared {
+struct alignas(16) Shared {  // histograms and slices are read 16 bytes at a time
   uint32_t hist[kDigits][kBins];  // of each digit (read by the cluster)
   uint32_t slice[kBins / 2];      // the cluster's sum of the bins this CTA adds up (read by the cluster)
   uint32_t warp_sum[32];
@@ -79,6 +80,8 @@ struct Shared {
   uint32_t digit;
   int left, equal;
 };
+static_assert(alignof(Shared) == 16 && offsetof(Shared, slice) % 16 == 0 && sizeof(Shared) % 16 == 0,
+              "16-byte accesses; the dynamic part may follow it");
 
 // sum of v over the threads before this one; the CTA's total in `all`.  `scratch` is free again
 // after the next barrier.
@@ -212,7 +215,7 @@ template <int NT, bool FUSED>
 __global__ void __launch_bounds__(NT, 1024 / NT) evict_kernel(EvictParams p, int C, int seg) {
   constexpr int kWarpsNT = NT / 32;
   // [seg] rank keys, then [seg / 32] words three times
-  extern __shared__ uint32_t keys[];
+  extern __shared__ __align__(16) uint32_t keys[];  // (written four at a time)
   uint32_t *stay = keys + seg;        // slots above T, then slots that stay, one bit each
   uint32_t *equal_w = stay + seg / 32;  // slots equal to T, then movers before each word
   uint32_t *hole0 = equal_w + seg / 32;  // holes before each word
