@@ -160,16 +160,6 @@ __device__ __forceinline__ void tmem_ld32_async(uint32_t addr, uint32_t (&r)[32]
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
-template <typename T> __device__ __forceinline__ uint32_t pack_pair(float a, float b);
-template <> __device__ __forceinline__ uint32_t pack_pair<__nv_bfloat16>(float a, float b) {
-  __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<uint32_t *>(&v);
-}
-template <> __device__ __forceinline__ uint32_t pack_pair<__half>(float a, float b) {
-  __half2 v = __floats2half2_rn(a, b);
-  return *reinterpret_cast<uint32_t *>(&v);
-}
-
 template <int G> struct RowsPerTok5 { static constexpr int value = G <= 1 ? 1 : G <= 2 ? 2 : G <= 4 ? 4 : 8; };
 
 struct Prefill5Params {
@@ -578,7 +568,7 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
                 b = ex2_approx(x1);
               }
               fadd2(ps[2 * (i & 3)], ps[2 * (i & 3) + 1], a, b);
-              pk[i] = pack_pair<T>(a, b);
+              pk[i] = pack2<T>(a, b);
             }
           };
           if constexpr (WIN && decltype(masked)::value) {
@@ -844,7 +834,7 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
       if (rw[i] < 0.f) continue;  // a wait ran out
       *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) +
                                  ((size_t(row0) + tk) * p.num_kv_heads * G + size_t(kvh) * G + hd) * D + ch * 4) =
-          make_uint2(pack_pair<T>(o[0], o[1]), pack_pair<T>(o[2], o[3]));
+          make_uint2(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]));
     }
     cluster_sync();  // no CTA leaves while another may read its shared memory
   } else if (all_ok) {
@@ -864,10 +854,10 @@ __global__ void __launch_bounds__(kThreads5, 1) paged_prefill_tc5_kernel(Prefill
 #pragma unroll
         for (int i = 0; i < 32; i += 8) {
           uint4 w;
-          w.x = pack_pair<T>(o[i] * inv, o[i + 1] * inv);
-          w.y = pack_pair<T>(o[i + 2] * inv, o[i + 3] * inv);
-          w.z = pack_pair<T>(o[i + 4] * inv, o[i + 5] * inv);
-          w.w = pack_pair<T>(o[i + 6] * inv, o[i + 7] * inv);
+          w.x = pack2<T>(o[i] * inv, o[i + 1] * inv);
+          w.y = pack2<T>(o[i + 2] * inv, o[i + 3] * inv);
+          w.z = pack2<T>(o[i + 4] * inv, o[i + 5] * inv);
+          w.w = pack2<T>(o[i + 6] * inv, o[i + 7] * inv);
           *reinterpret_cast<uint4 *>(stage + lane * (D * 2) + ((((c0 + i) >> 3) ^ (lane & 7)) << 4)) = w;
         }
       }
