@@ -48,11 +48,12 @@
 // 32-bit word per 32 columns, and only in the chunks that a row of the warp
 // does not see whole.  With fewer (tile, kv head) pairs than SMs a cluster
 // shares a tile's groups and joins its rows over distributed shared memory.
-// Measured: 4 x 4096 tokens, window 2048, 16/8 heads of 128, bf16: 265 us, 0.47
-// of the floor at the measured bf16 rate (2.36 us per 128-key group of both
-// halves, as the causal build, and ~7 us of fixed cost per CTA, 6.9 waves);
-// 512 tokens behind 7680, window 4096: 82 us on 32 CTAs, 35 us split over 4 each,
-// of which the join takes 5 (its 96 KB per CTA come at ~14 B a cycle).
+// Measured: 4 x 4096 tokens, window 2048, 16/8 heads of 128, bf16: 283 us a call
+// (260 in short bursts, before the power cap lowers the clock), 0.44 of the
+// floor at the measured bf16 rate (2.36 us per 128-key group of both halves, as
+// the causal build, and ~7 us of fixed cost per CTA, 6.9 waves); 512 tokens
+// behind 7680, window 4096: 82 us on 32 CTAs, 34 us split over 4 each, of which
+// the join takes 5 (its 96 KB per CTA come at ~14 B a cycle).
 //
 // Every wait is bounded (mbarrier polls that also watch a CTA abort flag);
 // on expiry the CTA records kStatusWaitTimeout, drains its MMAs and copies

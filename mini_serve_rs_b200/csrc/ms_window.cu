@@ -30,8 +30,10 @@
 // workspace, and the split depends on the call's shape only, so equal calls
 // give equal bits.
 // K3a needs the row's final maximum and sum before a score becomes a weight:
-// each CTA writes its raw scores to the workspace (they stay in L2) and reads
-// them back once the cluster has exchanged the maxima and sums.
+// each CTA writes its raw scores to the workspace and reads them back once the
+// cluster has exchanged the maxima and sums.  4 bytes per row, query head and
+// key: they stay in L2 for few rows (of 64 rows x 16 heads x 4608 keys, 19 MB,
+// 12 MB were written out; 155 us, 0.86 of the copy rate).
 #include <algorithm>
 #include <atomic>
 #include <cfloat>
