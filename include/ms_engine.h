@@ -451,9 +451,9 @@ int ms_prefill_tiles(const int32_t *seq_row0, const int32_t *seq_ntok, const int
  *    pages behind a window may have been freed or reused.  Keys that no row of
  *    a call's row (tile) sees may hold anything, NaN included.
  *  - A NaN in a query, or in a key or value that its row sees, makes that result
- *    NaN as the formula does (and every weight of that kv head and row).  In a
- *    tile a value that is not finite and that some of its rows see also spoils
- *    the others. */
+ *    NaN as the formula does; one in a query or key also every weight of that
+ *    kv head and row.  In a tile a value that is not finite and that some of
+ *    its rows see spoils the others too. */
 
 /* K3w: K3 with a sliding window and sink tokens.  Row t, at position p =
  * row_ctx[t] - 1, attends to the keys j <= p with p - j < window or j < sinks
